@@ -19,7 +19,7 @@
  *   - Return 0 on success, a negative errno-style code otherwise; no C++ exception crosses the boundary.
  *   - One ctx per device.  Calls on a ctx are stream-ordered on the hipStream_t passed in and are not
  *     re-entrant (the reference is single-threaded on the host, SURVEY.md section 8b "Threading").
- *   - All floating-point arrays are float32, ids are uint32 - the reference's dtypes.
+ *   - All floating-point arrays are float32, ids are uint32 - the reference's dtypes (the stand-alone operators also take float16 and bfloat16).
  */
 #ifndef NERFDS_H_
 #define NERFDS_H_
@@ -240,7 +240,8 @@ typedef struct nerfds_ctx nerfds_ctx;
 int nerfds_abi_version(void);
 /* sizeof the public structs as THIS library was compiled, for a binding to check its own declarations against (host only):
  * which = 0 nerfds_model_cfg, 1 nerfds_weights, 2 nerfds_camera, 3 nerfds_rays, 4 nerfds_extra, 5 nerfds_rand, 6 nerfds_out,
- * 7 nerfds_train_objective, 8 nerfds_train_numerics; anything else: -1. */
+ * 7 nerfds_train_objective, 8 nerfds_train_numerics, 9 / 10 nerfds_dense_forward_args / _backward_args, 11 / 12 nerfds_layer_norm_forward_args /
+ * _backward_args, 13 nerfds_matrix; anything else: -1. */
 int64_t nerfds_struct_size(int which);
 /* The arithmetic (NERFDS_PREC_BF16 / BF16X3 / F32 / F16) each network runs in under a NERFDS_PREC_* value of this build:
  * plan_out = {MaskMLP, SE3 warp field, hyper sheet, NerfMLP trunk (+ alpha head), rgb branch}.  Uniform for every value
@@ -434,6 +435,96 @@ int nerfds_trainer_nonfinite(nerfds_trainer* t);
  * L2 norm is at most grad_max_norm (if > 0).  Call between a NERFDS_TRAIN_GRADS_ONLY step (and the all-reduce) and nerfds_trainer_apply. */
 int nerfds_trainer_clip_gradients(nerfds_trainer* t, float grad_max_val, float grad_max_norm, void* hip_stream);
 const char* nerfds_trainer_last_error(const nerfds_trainer* t);
+
+/* ---- Stand-alone operators: a dense layer, a layer norm, the orthogonalisation of an update ----------------------------------------------------
+ * What a caller needs next to nerfds_trainer_forward / nerfds_render_rays_bwd to train layers of their own on rendered rays (nerfds_amd.layers and
+ * nerfds_amd.optim above them).  All array arguments are DEVICE pointers to row-major arrays of ONE element type per call; ld* are row strides in
+ * elements, so a view with unit stride along its last axis needs no copy; pointers need the alignment of their element type only.  Each call only
+ * enqueues work on hip_stream (capturable into a HIP graph), allocates nothing and leaves the thread's current device as it was.  A workspace
+ * belongs to its call until that work is done: two calls that may run at the same time (streams, replayed graphs) need one each.  Results do not
+ * depend on the order in which workgroups run: there are no atomics.  Error text: nerfds_last_error(NULL). */
+#define NERFDS_DTYPE_F32  0
+#define NERFDS_DTYPE_F16  1
+#define NERFDS_DTYPE_BF16 2
+#define NERFDS_ACT_NONE     0
+#define NERFDS_ACT_RELU     1
+#define NERFDS_ACT_SIGMOID  2
+#define NERFDS_ACT_SOFTPLUS 3
+#define NERFDS_ACT_SILU     4   /* z sigmoid(z) */
+#define NERFDS_ACT_GELU     5   /* z Phi(z), the erf form */
+/* y = act(x kernel + bias) + residual: nn.Dense (kernel [in][out]) with its epilogue in one kernel.  Products are accumulated in float32 and y is
+ * rounded once; float32 operands are multiplied as three bf16 parts each (float32-grade products; a non-finite operand gives a non-finite result,
+ * but an inf may arrive as NaN).  save (nerfds_dense_save_bytes bytes, or NULL for inference): what the backward needs of the pre-activation - one
+ * bit per element for relu, the pre-activation in the element type for the smooth activations, nothing for none. */
+typedef struct nerfds_dense_forward_args {
+  int32_t dtype, activation;
+  int64_t m;                          /* rows; 0 = nothing to do */
+  int32_t k, n;                       /* in, out; >= 1 */
+  const void* x; int64_t ldx;         /* [m][k] */
+  const void* kernel; int64_t ldk;    /* [k][n] */
+  const void* bias;                   /* [n] or NULL */
+  const void* residual; int64_t ldr;  /* [m][n] or NULL; ldr = 0: one row for all */
+  void* y; int64_t ldy;               /* [m][n], must not overlap an input (the residual in place is allowed: y == residual, ldy == ldr) */
+  void* save;
+} nerfds_dense_forward_args;
+/* dz = dy act'(z); dx = dz kernel^T, dkernel = x^T dz, dbias = column sums of dz; the gradient of the residual is dy itself.  dx / dkernel / dbias may
+ * be NULL (not computed).  For 16-bit tensors dz is rounded to their type between the slope and the products (none / relu: exact). */
+typedef struct nerfds_dense_backward_args {
+  int32_t dtype, activation;
+  int64_t m;                          /* 0: dkernel and dbias are cleared */
+  int32_t k, n;
+  const void* x; int64_t ldx;
+  const void* kernel; int64_t ldk;
+  const void* dy; int64_t lddy;       /* [m][n] */
+  const void* save;                   /* from the forward; NULL with NERFDS_ACT_NONE */
+  void* dx; int64_t lddx;             /* [m][k] */
+  void* dkernel;                      /* [k][n], contiguous */
+  void* dbias;                        /* [n] */
+  void* workspace; int64_t workspace_bytes;   /* >= nerfds_dense_backward_workspace(), 256-byte aligned */
+} nerfds_dense_backward_args;
+int64_t nerfds_dense_save_bytes(int32_t dtype, int32_t activation, int64_t m, int32_t n);                    /* negative: invalid argument */
+int64_t nerfds_dense_backward_workspace(int device, const nerfds_dense_backward_args* args);                /* bytes; the workspace fields are not read */
+int nerfds_dense_forward(int device, const nerfds_dense_forward_args* args, void* hip_stream);
+int nerfds_dense_backward(int device, const nerfds_dense_backward_args* args, void* hip_stream);
+/* Layer norm over the last axis of [m][d]: y = (x - mean) / sqrt(var + epsilon) * scale + bias (biased variance, two passes, float32 statistics).
+ * stats: [m][2] floats, mean and 1 / sqrt(var + epsilon) of each row, for the backward; NULL = not wanted.  A row with var = 0 and epsilon = 0 is NaN. */
+typedef struct nerfds_layer_norm_forward_args {
+  int32_t dtype, d;
+  int64_t m;
+  float epsilon;
+  const void* x; int64_t ldx;
+  const void* scale;                  /* [d] or NULL (1) */
+  const void* bias;                   /* [d] or NULL (0) */
+  void* y; int64_t ldy;               /* in place (y == x, ldy == ldx) is allowed */
+  float* stats;
+} nerfds_layer_norm_forward_args;
+typedef struct nerfds_layer_norm_backward_args {
+  int32_t dtype, d;
+  int64_t m;                          /* 0: dscale and dbias are cleared */
+  const void* x; int64_t ldx;
+  const void* scale;
+  const void* dy; int64_t lddy;
+  const float* stats;
+  void* dx; int64_t lddx;             /* or NULL */
+  void* dscale; void* dbias;          /* [d] or NULL */
+  void* workspace; int64_t workspace_bytes;   /* >= nerfds_layer_norm_backward_workspace(), 256-byte aligned */
+} nerfds_layer_norm_backward_args;
+int64_t nerfds_layer_norm_backward_workspace(int device, const nerfds_layer_norm_backward_args* args);
+int nerfds_layer_norm_forward(int device, const nerfds_layer_norm_forward_args* args, void* hip_stream);
+int nerfds_layer_norm_backward(int device, const nerfds_layer_norm_backward_args* args, void* hip_stream);
+/* Orthogonalises `count` matrices of any shapes: o ~ the orthogonal factor of u (u = Q S, singular values brought to about 1) by `steps` Newton-Schulz steps
+ *   X = u / |u|_F;   X <- a X + (b A + c A A) X,  A = X X^T  (on the short side),  (a, b, c) = (3.4445, -4.7750, 2.0315)
+ * float32-grade products whatever the element type.  A zero matrix gives zero; a non-finite element makes its own matrix NaN, no other.  o == u (same
+ * ld) is allowed; otherwise no o may overlap a u.  1 <= rows, cols <= NERFDS_ORTHO_MAX_DIM, 1 <= steps <= 16. */
+#define NERFDS_ORTHO_MAX_DIM 32768
+typedef struct nerfds_matrix {
+  const void* u; int64_t ldu;
+  void* o; int64_t ldo;
+  int32_t rows, cols;
+} nerfds_matrix;
+int64_t nerfds_orthogonalize_workspace(const nerfds_matrix* matrices, int32_t count);     /* bytes; negative: invalid argument */
+int nerfds_orthogonalize(int device, int32_t dtype, const nerfds_matrix* matrices, int32_t count, int32_t steps, void* workspace, int64_t workspace_bytes,
+                         void* hip_stream);
 
 /* Timing aid for bench.py: average device time (ms) of the render kernel launches recorded with HIP events
  * on the launch stream since the last reset; returns the number of launches measured. */

@@ -293,6 +293,11 @@ int64_t nerfds_struct_size(int which) {
     case 6: return sizeof(nerfds_out);
     case 7: return sizeof(nerfds_train_objective);
     case 8: return sizeof(nerfds_train_numerics);
+    case 9: return sizeof(nerfds_dense_forward_args);
+    case 10: return sizeof(nerfds_dense_backward_args);
+    case 11: return sizeof(nerfds_layer_norm_forward_args);
+    case 12: return sizeof(nerfds_layer_norm_backward_args);
+    case 13: return sizeof(nerfds_matrix);
     default: return -1;
   }
 }
@@ -309,6 +314,9 @@ int nerfds_precision_plan_level(uint32_t prec, int32_t level, int32_t plan_out[5
   plan_out[0] = pl.mask; plan_out[1] = pl.warp; plan_out[2] = pl.hyp; plan_out[3] = pl.trunk; plan_out[4] = pl.rgb;
   return NERFDS_OK;
 }
+
+// the message behind nerfds_last_error(NULL), for the entry points of operators.cpp
+void nerfds_set_last_error(const char* msg) { g_create_error = msg; }
 
 const char* nerfds_last_error(const nerfds_ctx* ctx) { return ctx ? ctx->err.c_str() : g_create_error.c_str(); }
 

@@ -125,6 +125,47 @@ class Out(C.Structure):
               ('sample_fine', C.c_void_p), ('sample_coarse', C.c_void_p)]
 
 
+# element types and activations of the stand-alone operators (NERFDS_DTYPE_* / NERFDS_ACT_*)
+ACTIVATIONS = {'none': 0, 'relu': 1, 'sigmoid': 2, 'softplus': 3, 'silu': 4, 'gelu': 5}
+
+
+def dtype_code(dtype) -> int:
+  """NERFDS_DTYPE_* of a torch dtype."""
+  import torch
+  codes = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+  if dtype not in codes:
+    raise ValueError(f'element type {dtype}: float32, float16 and bfloat16 are built')
+  return codes[dtype]
+
+
+class DenseForwardArgs(C.Structure):
+  _fields_ = [('dtype', C.c_int32), ('activation', C.c_int32), ('m', C.c_int64), ('k', C.c_int32), ('n', C.c_int32),
+              ('x', C.c_void_p), ('ldx', C.c_int64), ('kernel', C.c_void_p), ('ldk', C.c_int64), ('bias', C.c_void_p),
+              ('residual', C.c_void_p), ('ldr', C.c_int64), ('y', C.c_void_p), ('ldy', C.c_int64), ('save', C.c_void_p)]
+
+
+class DenseBackwardArgs(C.Structure):
+  _fields_ = [('dtype', C.c_int32), ('activation', C.c_int32), ('m', C.c_int64), ('k', C.c_int32), ('n', C.c_int32),
+              ('x', C.c_void_p), ('ldx', C.c_int64), ('kernel', C.c_void_p), ('ldk', C.c_int64), ('dy', C.c_void_p), ('lddy', C.c_int64),
+              ('save', C.c_void_p), ('dx', C.c_void_p), ('lddx', C.c_int64), ('dkernel', C.c_void_p), ('dbias', C.c_void_p),
+              ('workspace', C.c_void_p), ('workspace_bytes', C.c_int64)]
+
+
+class LayerNormForwardArgs(C.Structure):
+  _fields_ = [('dtype', C.c_int32), ('d', C.c_int32), ('m', C.c_int64), ('epsilon', C.c_float), ('x', C.c_void_p), ('ldx', C.c_int64),
+              ('scale', C.c_void_p), ('bias', C.c_void_p), ('y', C.c_void_p), ('ldy', C.c_int64), ('stats', C.c_void_p)]
+
+
+class LayerNormBackwardArgs(C.Structure):
+  _fields_ = [('dtype', C.c_int32), ('d', C.c_int32), ('m', C.c_int64), ('x', C.c_void_p), ('ldx', C.c_int64), ('scale', C.c_void_p),
+              ('dy', C.c_void_p), ('lddy', C.c_int64), ('stats', C.c_void_p), ('dx', C.c_void_p), ('lddx', C.c_int64),
+              ('dscale', C.c_void_p), ('dbias', C.c_void_p), ('workspace', C.c_void_p), ('workspace_bytes', C.c_int64)]
+
+
+class Matrix(C.Structure):
+  _fields_ = [('u', C.c_void_p), ('ldu', C.c_int64), ('o', C.c_void_p), ('ldo', C.c_int64), ('rows', C.c_int32), ('cols', C.c_int32)]
+
+
 # every symbol include/nerfds.h declares
 SYMBOLS = ('nerfds_abi_version', 'nerfds_struct_size', 'nerfds_precision_plan', 'nerfds_precision_plan_level', 'nerfds_ctx_create', 'nerfds_ctx_load_weights', 'nerfds_render_rays',
            'nerfds_encode_embed', 'nerfds_ctx_destroy', 'nerfds_last_error', 'nerfds_kernel_time_ms', 'nerfds_pack_stream_bytes', 'nerfds_pack_stream_bytes_level',
@@ -133,7 +174,9 @@ SYMBOLS = ('nerfds_abi_version', 'nerfds_struct_size', 'nerfds_precision_plan', 
            'nerfds_trainer_num_leaves', 'nerfds_trainer_leaf', 'nerfds_trainer_params', 'nerfds_trainer_grads',
            'nerfds_trainer_download', 'nerfds_trainer_upload', 'nerfds_trainer_reset_optimizer', 'nerfds_trainer_step', 'nerfds_trainer_apply', 'nerfds_trainer_clip_gradients', 'nerfds_trainer_target_norm',
            'nerfds_trainer_last_error', 'nerfds_trainer_debug_read', 'nerfds_trainer_nonfinite', 'nerfds_trainer_set_step', 'nerfds_trainer_get_step', 'nerfds_trainer_set_loss_scale_adjust', 'nerfds_trainer_set_numerics', 'nerfds_trainer_get_numerics', 'nerfds_trainer_overflow_sources', 'nerfds_trainer_forward', 'nerfds_render_rays_bwd',
-           'nerfds_debug_lds_attr_first_use')
+           'nerfds_debug_lds_attr_first_use',
+           'nerfds_dense_save_bytes', 'nerfds_dense_backward_workspace', 'nerfds_dense_forward', 'nerfds_dense_backward', 'nerfds_layer_norm_forward',
+           'nerfds_layer_norm_backward_workspace', 'nerfds_layer_norm_backward', 'nerfds_orthogonalize_workspace', 'nerfds_orthogonalize')
 
 _lib = None
 
@@ -181,7 +224,20 @@ def load():
     raise RuntimeError('libnerfds_hip.so ABI version mismatch: rebuild')
   lib.nerfds_struct_size.argtypes = [C.c_int]
   lib.nerfds_struct_size.restype = C.c_int64
-  for which, st in enumerate((ModelCfg, Weights, CameraStruct, Rays, Extra, Rand, Out)):      # the ctypes mirrors against the library's own sizeof
+  lib.nerfds_dense_save_bytes.argtypes = [C.c_int32, C.c_int32, C.c_int64, C.c_int32]
+  lib.nerfds_dense_backward_workspace.argtypes = [C.c_int, C.POINTER(DenseBackwardArgs)]
+  lib.nerfds_dense_forward.argtypes = [C.c_int, C.POINTER(DenseForwardArgs), C.c_void_p]
+  lib.nerfds_dense_backward.argtypes = [C.c_int, C.POINTER(DenseBackwardArgs), C.c_void_p]
+  lib.nerfds_layer_norm_forward.argtypes = [C.c_int, C.POINTER(LayerNormForwardArgs), C.c_void_p]
+  lib.nerfds_layer_norm_backward_workspace.argtypes = [C.c_int, C.POINTER(LayerNormBackwardArgs)]
+  lib.nerfds_layer_norm_backward.argtypes = [C.c_int, C.POINTER(LayerNormBackwardArgs), C.c_void_p]
+  lib.nerfds_orthogonalize_workspace.argtypes = [C.POINTER(Matrix), C.c_int32]
+  lib.nerfds_orthogonalize.argtypes = [C.c_int, C.c_int32, C.POINTER(Matrix), C.c_int32, C.c_int32, C.c_void_p, C.c_int64, C.c_void_p]
+  for f in (lib.nerfds_dense_save_bytes, lib.nerfds_dense_backward_workspace, lib.nerfds_layer_norm_backward_workspace, lib.nerfds_orthogonalize_workspace):
+    f.restype = C.c_int64
+  structs = {i: st for i, st in enumerate((ModelCfg, Weights, CameraStruct, Rays, Extra, Rand, Out))}
+  structs.update({9: DenseForwardArgs, 10: DenseBackwardArgs, 11: LayerNormForwardArgs, 12: LayerNormBackwardArgs, 13: Matrix})
+  for which, st in structs.items():      # the ctypes mirrors against the library's own sizeof
     if lib.nerfds_struct_size(which) != C.sizeof(st):
       raise RuntimeError(f'{st.__name__}: ctypes declares {C.sizeof(st)} bytes, libnerfds_hip.so has {lib.nerfds_struct_size(which)} (include/nerfds.h changed?)')
   _lib = lib

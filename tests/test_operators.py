@@ -1,0 +1,577 @@
+"""The stand-alone operators (nerfds_amd.layers, nerfds_amd.optim) against their definitions in 64 bits, and their refusals.
+
+Tolerances count roundings: u = half a step of the element type for each rounding to it, and 2^-24 for each float32 operation of the longest chain an element
+passes through, times the sum of magnitudes it is taken of."""
+import ctypes as C
+import math
+
+import pytest
+import torch
+
+from nerfds_amd import _native as N
+from nerfds_amd import layers, optim
+
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+E24 = 2.0 ** -24
+SMOOTH = ('sigmoid', 'softplus', 'silu', 'gelu')
+
+
+def half_step(t):
+  return torch.finfo(t).eps / 2
+
+
+def tiny(t):      # half the spacing of the subnormals: what a rounding may lose where values underflow
+  return torch.finfo(t).smallest_normal * torch.finfo(t).eps / 2
+
+
+def make(*shape, t=F32, seed=0, scale=1.0, shift=0.0, grid=None):
+  g = torch.Generator().manual_seed(seed)
+  v = torch.randn(shape, generator=g, dtype=torch.float64) * scale + shift
+  if grid is not None:
+    v = (v.clamp(-2, 2) / grid).round() * grid
+  return v.to(t)
+
+
+def dev(*ts):
+  return [None if v is None else v.cuda() for v in ts]
+
+
+def act64(z, act):
+  """(act(z), act'(z), a bound of |act''|)."""
+  s = torch.sigmoid(z)
+  if act == 'none':
+    return z, torch.ones_like(z), 0.0
+  if act == 'relu':
+    return z.clamp_min(0), (z > 0).double(), 0.0
+  if act == 'sigmoid':
+    return s, s * (1 - s), 0.1
+  if act == 'softplus':
+    return torch.logaddexp(z, torch.zeros_like(z)), s, 0.25
+  if act == 'silu':
+    return z * s, s * (1 + z * (1 - s)), 0.5
+  cdf = 0.5 * torch.erfc(-z / math.sqrt(2))
+  return z * cdf, cdf + z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi), 0.8
+
+
+def dense64(x, w, b, r, act, dy=None):
+  """{name: (value, bound of the error)} of the dense layer for inputs of x's type."""
+  t = x.dtype
+  u = half_step(t)
+  x, w = x.double(), w.double()
+  k, n, m = x.shape[1], w.shape[1], x.shape[0]
+  z, mag = x @ w, x.abs() @ w.abs()
+  if b is not None:
+    z, mag = z + b.double(), mag + b.double().abs()
+  ez = (k + 8) * E24 * mag                     # float32 accumulation (and, for float32 operands, the dropped products)
+  y, slope, curve = act64(z, act)
+  ey = 1.2 * ez + 16 * E24 * (y.abs() + mag * 0)      # slopes are at most 1.13; the activation's own few float32 roundings
+  if r is not None:
+    y = y + r.double()
+    ey = ey + 2 * E24 * (y.abs() + r.double().abs())
+  out = {'y': (y, ey + u * y.abs() + tiny(t) + E24 * 1e-6)}
+  if dy is None:
+    return out
+  dy = dy.double()
+  dz = dy * slope
+  edz = torch.zeros_like(dz)
+  if act in SMOOTH:      # z is kept in the tensors' type, dz rounded to it
+    edz = dy.abs() * (curve * (ez + u * z.abs()) + 16 * E24) + u * dz.abs() + tiny(t)
+  def product(a, e, b2, length):
+    return a @ b2, e @ b2.abs() + (length + 8) * E24 * (a.abs() @ b2.abs())
+  for name, (v, e) in {'dx': product(dz, edz, w.t(), n), 'dkernel': tuple(q.t() for q in product(dz.t(), edz.t(), x, m))}.items():
+    out[name] = (v, e + u * v.abs() + tiny(t))
+  v = dz.sum(0)
+  out['db'] = (v, edz.sum(0) + (m + 8) * E24 * dz.abs().sum(0) + u * v.abs() + tiny(t))
+  return out
+
+
+def close(got, want, what=''):
+  v, e = want
+  got = got.detach().cpu().double().reshape(v.shape)
+  bad = (got - v).abs() > e
+  assert torch.isfinite(got).all() and not bad.any(), (what, int(bad.sum()), float(((got - v).abs() / e.clamp_min(1e-300)).max()))
+
+
+SHAPES = [(1, 1, 1), (1, 256, 256), (3, 7, 5), (2, 64, 3), (17, 130, 9), (130, 33, 131), (257, 560, 128), (64, 64, 64), (129, 128, 300), (1025, 45, 64)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('t', [F32, F16, BF16], ids=['f32', 'f16', 'bf16'])
+@pytest.mark.parametrize('i', range(len(SHAPES)), ids=['x'.join(map(str, s)) for s in SHAPES])
+def test_dense_and_its_gradients(i, t):
+  m, k, n = SHAPES[i]
+  for j, act in enumerate(N.ACTIVATIONS):
+    bias, residual = (i + j) % 3 != 0, (i + j) % 2 == 0
+    # relu: values on a grid whose products and sums float32 holds exactly, so that no rounding moves a pre-activation across 0 (many ARE 0)
+    grid = 0.25 if act == 'relu' else None
+    x, w = make(m, k, t=t, seed=1, grid=grid), make(k, n, t=t, seed=2, scale=1.0 if grid else k ** -0.5, grid=grid)
+    b = make(n, t=t, seed=3, grid=grid) if bias else None
+    r = make(m, n, t=t, seed=4) if residual else None
+    dy = make(m, n, t=t, seed=5)
+    want = dense64(x, w, b, r, act, dy)
+    leaves = [v.requires_grad_(True) if v is not None else None for v in dev(x, w, b, r)]
+    y = layers.dense(leaves[0], leaves[1], leaves[2], activation=act, residual=leaves[3])
+    close(y, want['y'], act)
+    close(layers.dense(*dev(x, w, b), activation=act, residual=dev(r)[0]), want['y'], act)
+    y.backward(dy.cuda())
+    for name, v in zip(('dx', 'dkernel', 'db'), leaves):
+      if v is not None:
+        close(v.grad, want[name], (act, name))
+    if r is not None:
+      assert torch.equal(leaves[3].grad.cpu(), dy)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('t', [F32, BF16], ids=['f32', 'bf16'])
+def test_dense_at_sizes_with_many_tiles_and_splits(t):
+  for m, k, n, act in ((20011, 172, 131, 'relu'), (4099, 520, 1031, 'gelu'), (300, 1500, 70, 'none')):
+    grid = 0.25 if act == 'relu' else None
+    x, w, dy = make(m, k, t=t, seed=6, grid=grid), make(k, n, t=t, seed=7, scale=1.0 if grid else k ** -0.5, grid=grid), make(m, n, t=t, seed=8)
+    b = make(n, t=t, seed=9, grid=grid)
+    want = dense64(x, w, b, None, act, dy)
+    y, saved = layers.dense_forward(*dev(x, w, b), activation=act)
+    close(y, want['y'])
+    got = layers.dense_backward(*dev(dy, x, w), saved, act)
+    for name, g in zip(('dx', 'dkernel', 'db'), got):
+      close(g, want[name], (m, name))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('t', [F32, F16], ids=['f32', 'f16'])
+def test_dense_takes_views_expanded_residuals_and_leading_axes(t):
+  m, k, n = 35, 37, 41
+  big, wbig, gbig = make(m, 3 * k + 1, t=t, seed=1).cuda(), make(k, 2 * n + 3, t=t, seed=2).cuda(), make(n, m, t=t, seed=3).cuda()
+  x, w, dy = big[:, k + 1:2 * k + 1], wbig[:, 1:n + 1], gbig.t()      # odd offsets, padded rows, a transposed cotangent
+  r = make(n, t=t, seed=4).cuda().expand(m, n)                        # one row for all
+  want = dense64(x.cpu(), w.cpu(), None, r.cpu(), 'silu', dy.cpu())
+  y, saved = layers.dense_forward(x, w, None, 'silu', r)
+  close(y, want['y'])
+  for name, g in zip(('dx', 'dkernel', 'db'), layers.dense_backward(dy, x, w, saved, 'silu')):
+    close(g, want[name], name)
+  close(layers.dense(x.reshape(5, 7, k), w.t().contiguous().t(), None, 'silu', r.reshape(5, 7, n)), want['y'])
+  shared = make(n, t=t, seed=4).cuda().requires_grad_(True)           # the gradient of a broadcast input is summed over the rows
+  layers.dense(x, w, None, 'silu', shared.expand(m, n)).backward(dy)
+  v = dy.cpu().double().sum(0)
+  close(shared.grad, (v, (half_step(t) + m * E24) * dy.cpu().double().abs().sum(0)))
+
+
+@pytest.mark.gpu
+def test_dense_computes_what_is_asked_for_and_handles_no_rows():
+  x, w, b, dy = dev(make(70, 40, seed=1), make(40, 50, seed=2), make(50, seed=3), make(70, 50, seed=4))
+  y, saved = layers.dense_forward(x, w, b, 'softplus')
+  full = layers.dense_backward(dy, x, w, saved, 'softplus')
+  for need in range(8):
+    flags = [bool(need >> i & 1) for i in range(3)]
+    got = layers.dense_backward(dy, x, w, saved, 'softplus', need_dx=flags[0], need_dkernel=flags[1], need_dbias=flags[2])
+    for f, g, ref in zip(flags, got, full):
+      assert (g is None) != f and (g is None or torch.equal(g, ref))
+  for act in ('none', 'relu', 'gelu'):
+    e = x[:0].clone().requires_grad_(True)
+    wl, bl = w.clone().requires_grad_(True), b.clone().requires_grad_(True)
+    out = layers.dense(e, wl, bl, activation=act)
+    assert out.shape == (0, 50)
+    out.sum().backward()
+    assert e.grad.shape == (0, 40) and not wl.grad.any() and not bl.grad.any()
+
+
+@pytest.mark.gpu
+def test_dense_gradient_against_differences():
+  x, w, b, dy = make(9, 12, seed=1), make(12, 10, seed=2, scale=0.3), make(10, seed=3), make(9, 10, seed=4)
+  for act in ('sigmoid', 'softplus', 'silu', 'gelu'):
+    leaves = [v.requires_grad_(True) for v in dev(x, w, b)]
+    layers.dense(*leaves, activation=act).backward(dy.cuda())
+    for i, v in enumerate((x, w, b)):
+      d = make(*v.shape, seed=7 + i).double()
+      h = 1e-5
+      at = lambda q: float((act64((x.double() + (q * d if i == 0 else 0)) @ (w.double() + (q * d if i == 1 else 0)) + b.double() + (q * d if i == 2 else 0), act)[0] * dy.double()).sum())
+      slope = (at(h) - at(-h)) / (2 * h)
+      got = float((leaves[i].grad.cpu().double() * d).sum())
+      assert abs(got - slope) < 1e-4 * (1 + abs(slope)), (act, i, got, slope)      # h^2 of the difference (~1e-9) and float32 over some 100 terms
+
+
+@pytest.mark.gpu
+def test_dense_non_finite_inputs_stay_in_their_rows():
+  for t in (F32, F16, BF16):
+    x, w = make(140, 50, t=t, seed=1), make(50, 20, t=t, seed=2)
+    x[3, 49], x[130, 0] = float('nan'), float('inf')
+    y = layers.dense(*dev(x, w), activation='relu').cpu()
+    rows = ~torch.isfinite(y).all(1)
+    assert not torch.isfinite(y[3]).any() and rows[3] and rows[130] and int(rows.sum()) == 2
+
+
+@pytest.mark.gpu
+def test_dense_offsets_beyond_32_bits():
+  m, k, n = (1 << 32) // 64 + 77, 64, 8      # more than 2^32 elements of x
+  w = make(k, n, t=BF16, seed=1).cuda()
+  x = torch.zeros((m, k), dtype=BF16, device='cuda')
+  x[-130:] = make(130, k, t=BF16, seed=2).cuda()
+  want = dense64(x[-130:].cpu(), w.cpu(), None, None, 'none', torch.ones(130, n, dtype=BF16))
+  y = layers.dense(x, w)
+  close(y[-130:], want['y'])
+  assert not y[:1000].any()
+  dx, dkernel, _ = layers.dense_backward(torch.ones_like(y), x, w, None, need_dbias=False)
+  close(dx[-130:], want['dx'])
+  close(dkernel, want['dkernel'])
+
+
+# ---- layer norm ---------------------------------------------------------------------------------------------------------------------------------
+def norm64(x, scale, bias, eps, dy):
+  t = x.dtype
+  u = half_step(t)
+  x, d = x.double(), x.shape[1]
+  one = torch.ones(d, dtype=torch.float64)
+  w = one if scale is None else scale.double()
+  b = 0 * one if bias is None else bias.double()
+  chain = 64                                        # a lane adds at most 34 elements, then 8 partial sums
+  mu = x.mean(1, keepdim=True)
+  emu = (chain + 2) * E24 * x.abs().mean(1, keepdim=True)
+  c = x - mu
+  rstd = 1 / (c.square().mean(1, keepdim=True) + eps).sqrt()
+  rel = (chain + 8) * E24 + emu * emu * rstd * rstd + 2 * E24 * c.abs().max(1, keepdim=True).values * rstd     # of rstd: the sum, emu enters squared
+  xh = c * rstd
+  ex = rstd * (emu + E24 * (x.abs() + mu.abs())) + xh.abs() * (rel + 2 * E24)
+  y = xh * w + b
+  out = {'y': (y, ex * w.abs() + 4 * E24 * (y.abs() + b.abs()) + u * y.abs() + tiny(t) + 1e-300)}
+  dy = dy.double()
+  h = dy * w
+  m1, m2 = h.mean(1, keepdim=True), (h * xh).mean(1, keepdim=True)
+  e1 = (chain + 2) * E24 * h.abs().mean(1, keepdim=True)
+  e2 = (chain + 4) * E24 * (h * xh).abs().mean(1, keepdim=True) + (h.abs() * ex).mean(1, keepdim=True)
+  dx = rstd * (h - m1 - xh * m2)
+  edx = rstd * (e1 + ex * m2.abs() + xh.abs() * e2 + 4 * E24 * (h.abs() + m1.abs() + (xh * m2).abs())) + dx.abs() * (rel + 2 * E24)
+  out['dx'] = (dx, edx + u * dx.abs() + tiny(t) + 1e-300)
+  rows = min(x.shape[0], 512) + 64                   # rows a lane adds, then the partial sums
+  v = (dy * xh).sum(0)
+  out['dscale'] = (v, (dy.abs() * ex).sum(0) + rows * E24 * (dy * xh).abs().sum(0) + u * v.abs() + tiny(t) + 1e-300)
+  v = dy.sum(0)
+  out['dbias'] = (v, rows * E24 * dy.abs().sum(0) + u * v.abs() + tiny(t) + 1e-300)
+  return out
+
+
+NORM_SHAPES = [(1, 1), (5, 1), (3, 2), (1, 256), (33, 8), (7, 33), (70, 64), (31, 65), (9, 129), (300, 256), (6, 511), (5, 513), (13, 1023), (4, 1025), (3, 2049), (3, 4100),
+               (2, 8192), (2, 8200), (3000, 24)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('t', [F32, F16, BF16], ids=['f32', 'f16', 'bf16'])
+@pytest.mark.parametrize('i', range(len(NORM_SHAPES)), ids=['x'.join(map(str, s)) for s in NORM_SHAPES])
+def test_layer_norm_and_its_gradients(i, t):
+  m, d = NORM_SHAPES[i]
+  x, dy = make(m, d, t=t, seed=1, scale=1.5, shift=0.5), make(m, d, t=t, seed=2)
+  scale = make(d, t=t, seed=3, scale=0.2, shift=1.0) if i % 3 else None
+  bias = make(d, t=t, seed=4) if i % 2 else None
+  want = norm64(x, scale, bias, 1e-6, dy)
+  leaves = [v.requires_grad_(True) if v is not None else None for v in dev(x, scale, bias)]
+  y = layers.layer_norm(*leaves)
+  close(y, want['y'])
+  close(layers.layer_norm(*dev(x, scale, bias)), want['y'])
+  y.backward(dy.cuda())
+  for name, v in zip(('dx', 'dscale', 'dbias'), leaves):
+    if v is not None:
+      close(v.grad, want[name], name)
+
+
+@pytest.mark.gpu
+def test_layer_norm_far_mean_constant_rows_views_and_no_rows():
+  x = make(40, 300, seed=1, scale=1e-2, shift=100.0)      # a difference of squares would keep no digit of this variance
+  x[7] = 0.1                                               # a constant row: bias comes out
+  dy = make(40, 300, seed=2)
+  want = norm64(x, None, None, 1e-6, dy)
+  y, stats = layers.layer_norm_forward(x.cuda())
+  close(y, want['y'])
+  close(layers.layer_norm_backward(*dev(dy, x), None, stats, need_dscale=False, need_dbias=False)[0], want['dx'])
+  big = make(20, 101, seed=3).cuda()
+  v = big[:, 1:98]
+  want = norm64(v.cpu(), None, None, 0.1, v.cpu())
+  y, stats = layers.layer_norm_forward(v, epsilon=0.1)
+  close(y, want['y'])
+  close(layers.layer_norm_backward(v, v, None, stats)[0], want['dx'])
+  close(layers.layer_norm(v.reshape(4, 5, 97), epsilon=0.1), want['y'])
+  s = torch.ones(97, device='cuda').requires_grad_(True)
+  e = v[:0].clone().requires_grad_(True)
+  layers.layer_norm(e, s).sum().backward()
+  assert e.grad.shape == (0, 97) and not s.grad.any()
+
+
+@pytest.mark.gpu
+def test_layer_norm_gradient_against_differences_and_what_is_asked_for():
+  x, s, b, dy = make(6, 20, seed=1), make(20, seed=2, shift=1.0), make(20, seed=3), make(6, 20, seed=4)
+  leaves = [v.requires_grad_(True) for v in dev(x, s, b)]
+  layers.layer_norm(*leaves).backward(dy.cuda())
+
+  def f(xx, ss, bb):
+    return float((norm64_value(xx, ss, bb) * dy.double()).sum())
+  def norm64_value(xx, ss, bb):
+    c = xx - xx.mean(1, keepdim=True)
+    return c / (c.square().mean(1, keepdim=True) + 1e-6).sqrt() * ss + bb
+  for i, v in enumerate((x, s, b)):
+    d = make(*v.shape, seed=7 + i).double()
+    args = [q.double() for q in (x, s, b)]
+    hi, lo = list(args), list(args)
+    hi[i], lo[i] = args[i] + 1e-5 * d, args[i] - 1e-5 * d
+    slope = (f(*hi) - f(*lo)) / 2e-5
+    got = float((leaves[i].grad.cpu().double() * d).sum())
+    assert abs(got - slope) < 1e-4 * (1 + abs(slope)), (i, got, slope)
+  _, stats = layers.layer_norm_forward(*dev(x, s, b))
+  full = layers.layer_norm_backward(*dev(dy, x, s), stats)
+  for need in range(8):
+    flags = [bool(need >> i & 1) for i in range(3)]
+    got = layers.layer_norm_backward(*dev(dy, x, s), stats, need_dx=flags[0], need_dscale=flags[1], need_dbias=flags[2])
+    for fl, g, ref in zip(flags, got, full):
+      assert (g is None) != fl and (g is None or torch.equal(g, ref))
+
+
+# ---- orthogonalised updates ------------------------------------------------------------------------------------------------------------------------
+def ortho64(u, steps=5):
+  x = u.double()
+  n = x.norm()
+  x = x / n if n > 1e-30 else x * 0
+  tall = x.shape[0] > x.shape[1]
+  x = x.t() if tall else x
+  for _ in range(steps):
+    a = x @ x.t()
+    x = 3.4445 * x + (-4.7750 * a + 2.0315 * a @ a) @ x
+  return x.t() if tall else x
+
+
+# Relative error of the result (2-norm over all elements): a singular value and its error grow by the same factor while the value is small, so relative
+# errors add up over the 3 products of each of the steps, each 2^-22 (two f16 planes a side) times |a| + |b| + |c| = 10
+def ortho_bound(t, steps=5):
+  return steps * 3 * 10 * 2.0 ** -22 + (half_step(t) if t != F32 else 0.0)
+
+
+ORTHO_SHAPES = [(1, 1), (1, 7), (9, 1), (3, 5), (64, 64), (63, 65), (65, 64), (128, 45), (256, 256), (130, 517), (560, 128), (20, 3001)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('t', [F32, F16, BF16], ids=['f32', 'f16', 'bf16'])
+def test_orthogonalize_alone_and_in_one_call(t):
+  mats = [make(r, c, t=t, seed=10 + i, scale=0.01) for i, (r, c) in enumerate(ORTHO_SHAPES)]
+  mats[4] = (make(64, 6, seed=1) @ make(6, 64, seed=2)).to(t)             # low rank: most singular values are roundings
+  got = optim.orthogonalize(dev(*mats))
+  for u, o in zip(mats, got):
+    want = ortho64(u)
+    err = float((o.cpu().double() - want).norm() / want.norm())
+    assert o.dtype == t and o.shape == u.shape and err < ortho_bound(t), (tuple(u.shape), err)
+    assert torch.equal(optim.orthogonalize(u.cuda()), o), tuple(u.shape)        # the same bits alone and among others
+  s = torch.linalg.svdvals(got[8].double().cpu())
+  assert float(s.max()) < 1.21 and float(s[:200].min()) > 0.6
+
+
+@pytest.mark.gpu
+def test_orthogonalize_extreme_values_zero_and_non_finite_matrices():
+  u = make(70, 90, seed=1)
+  want = ortho64(u)
+  one = torch.zeros(70, 90)
+  one[3, 80] = -1e-20
+  bad = u.clone()
+  bad[0, 0] = float('inf')
+  got = optim.orthogonalize(dev(u * 1e30, u * 1e-25, torch.zeros(70, 90), bad, one, u))
+  for o in (got[0], got[1], got[5]):
+    assert float((o.cpu().double() - want).norm() / want.norm()) < ortho_bound(F32) + 2 * E24
+  assert not got[2].any() and torch.isnan(got[3]).all()
+  assert float((got[4].cpu().double() - ortho64(one)).abs().max()) < 1e-4
+  for steps in (1, 2, 7, 16):
+    want = ortho64(u, steps)
+    assert float((optim.orthogonalize(u.cuda(), steps=steps).cpu().double() - want).norm() / want.norm()) < ortho_bound(F32, steps) * 4
+
+
+@pytest.mark.gpu
+def test_orthogonalize_many_matrices_views_and_empty_ones():
+  big = make(300, 400, seed=1).cuda()
+  mats = [big[i:i + 5 + i % 30, 3 * i:3 * i + 40 - i % 17] for i in range(70)] + [big.t()[:50, :60], big[:0], big[:, :0]]     # two launches' worth
+  got = optim.orthogonalize(mats)
+  for u, o in zip(mats, got):
+    assert o.shape == u.shape and o.is_contiguous()
+    if u.numel():
+      want = ortho64(u.cpu())
+      assert float((o.cpu().double() - want).norm() / want.norm()) < ortho_bound(F32), tuple(u.shape)
+  assert optim.orthogonalize([]) == []
+
+
+# ---- streams, graphs, repetition -------------------------------------------------------------------------------------------------------------------
+def _block(p, dy):
+  """A pre-norm residual block, its gradients and their orthogonalisation, as a user's step runs them - without autograd, so it can be captured."""
+  h, stats = layers.layer_norm_forward(p['x'], p['s'], p['b'])
+  a, saved = layers.dense_forward(h, p['w1'], p['b1'], 'gelu')
+  y, _ = layers.dense_forward(a, p['w2'], None, 'none', residual=p['x'])
+  da, dw2, _ = layers.dense_backward(dy, a, p['w2'], None, need_dbias=False)
+  dh, dw1, db1 = layers.dense_backward(da, h, p['w1'], saved, 'gelu')
+  dx, ds, db = layers.layer_norm_backward(dh, p['x'], p['s'], stats)
+  o1, o2 = optim.orthogonalize([dw1, dw2])
+  return y, dx + dy, ds, db, dw1, db1, dw2, o1, o2
+
+
+def _block_state(seed, t=F32, m=200, d=96, hidden=160):
+  p = dict(x=make(m, d, t=t, seed=seed), s=make(d, t=t, seed=seed + 1, shift=1.0), b=make(d, t=t, seed=seed + 2), w1=make(d, hidden, t=t, seed=seed + 3, scale=0.1),
+           b1=make(hidden, t=t, seed=seed + 4), w2=make(hidden, d, t=t, seed=seed + 5, scale=0.1))
+  return {k: v.cuda() for k, v in p.items()}, make(m, d, t=t, seed=seed + 6).cuda()
+
+
+@pytest.mark.gpu
+def test_block_against_autograd_in_64_bits_and_repeats_bit_for_bit():
+  p, dy = _block_state(1)
+  q = {k: v.cpu().double().requires_grad_(True) for k, v in p.items()}
+  c = q['x'] - q['x'].mean(1, keepdim=True)
+  h = c / (c.square().mean(1, keepdim=True) + 1e-6).sqrt() * q['s'] + q['b']
+  y = q['x'] + torch.nn.functional.gelu(h @ q['w1'] + q['b1']) @ q['w2']
+  y.backward(dy.cpu().double())
+  got = _block(p, dy)
+  want = [y] + [q[k].grad for k in ('x', 's', 'b', 'w1', 'b1', 'w2')] + [ortho64(q[k].grad) for k in ('w1', 'w2')]
+  for i, (g, v) in enumerate(zip(got, want)):      # five float32 stages, the longest sum 200 terms: 5 x 200 x 2^-24 of the norm at the most
+    assert float((g.cpu().double() - v).norm() / v.norm()) < 1000 * E24, i
+  leaves = {k: v.clone().requires_grad_(True) for k, v in p.items()}
+  a = layers.dense(layers.layer_norm(leaves['x'], leaves['s'], leaves['b']), leaves['w1'], leaves['b1'], activation='gelu')
+  layers.dense(a, leaves['w2'], residual=leaves['x']).backward(dy)
+  for k, v in zip(('s', 'b', 'w1', 'b1', 'w2'), got[2:7]):
+    assert torch.equal(leaves[k].grad, v), k
+  for _ in range(3):
+    for a, b in zip(_block(p, dy), got):
+      assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_two_captured_graphs_replay_with_eager_work_between():
+  states = [_block_state(1), _block_state(20)]
+  eager = [[v.clone() for v in _block(*s)] for s in states]
+  graphs = []
+  side = torch.cuda.Stream()
+  for s in states:
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+      _block(*s)
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+      out = _block(*s)
+    graphs.append((g, out))
+  for turn in range(3):
+    for (g, out), want in zip(graphs, eager):
+      for o in out:
+        o.zero_()
+      g.replay()
+      fresh = _block(*states[turn % 2])
+      torch.cuda.synchronize()
+      for a, b in zip(out, want):
+        assert torch.equal(a, b)
+      for a, b in zip(fresh, eager[turn % 2]):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_other_streams_and_the_current_device():
+  states = [_block_state(40 + i) for i in range(3)]
+  want = [_block(*s) for s in states]
+  torch.cuda.synchronize()
+  streams = [torch.cuda.Stream() for _ in states]
+  got = []
+  for st, s in zip(streams, states):
+    with torch.cuda.stream(st):
+      got.append(_block(*s))
+  torch.cuda.synchronize()
+  for a, b in zip(got, want):
+    for x, y in zip(a, b):
+      assert torch.equal(x, y)
+  assert torch.cuda.current_device() == 0
+  if torch.cuda.device_count() > 1:
+    x = make(5, 6, seed=1)
+    assert torch.equal(layers.layer_norm(x.to('cuda:1')).cpu(), layers.layer_norm(x.cuda()).cpu()) and torch.cuda.current_device() == 0
+
+
+# ---- refusals (no GPU needed: every check comes before the device) -------------------------------------------------------------------------------------
+def test_python_refusals():
+  x = torch.zeros(4, 8)
+  for f in (lambda: layers.dense(x, torch.zeros(8, 3)), lambda: layers.layer_norm(x), lambda: optim.orthogonalize(x), lambda: optim.orthogonalize([x])):
+    with pytest.raises(RuntimeError, match='no CPU path'):
+      f()
+  with pytest.raises(ValueError, match='steps'):
+    optim.orthogonalize(x, steps=0)
+  with pytest.raises(ValueError, match='2-d'):
+    optim.orthogonalize([torch.zeros(3)])
+  with pytest.raises(ValueError, match='at least one axis'):
+    layers.dense(torch.tensor(1.0), torch.zeros(1, 1))
+
+
+@pytest.mark.gpu
+def test_python_refusals_on_the_gpu():
+  x, w = torch.zeros(4, 8, device='cuda'), torch.zeros(8, 3, device='cuda')
+  cases = [(lambda: layers.dense(x, w.half()), 'kernel must be'), (lambda: layers.dense(x, w.cpu()), 'kernel must be'), (lambda: layers.dense(x, w[:7]), 'does not fit'),
+           (lambda: layers.dense(x, w[:, :0]), 'does not fit'), (lambda: layers.dense(x.double(), w.double()), 'element type'), (lambda: layers.dense(x, w, activation='tanh'), 'activation'),
+           (lambda: layers.dense(x, w, torch.zeros(4, device='cuda')), 'bias'), (lambda: layers.dense(x, w, residual=x), 'residual'),
+           (lambda: layers.dense_backward(x[:, :3], x, w, None, 'relu'), 'saved'), (lambda: layers.dense_backward(x, x, w, None), 'dy'),
+           (lambda: layers.layer_norm(x, w[:, 0][:3]), 'scale'), (lambda: layers.layer_norm(x, epsilon=-1.0), 'epsilon'), (lambda: layers.layer_norm(x[:, :0]), 'last axis'),
+           (lambda: layers.layer_norm(x, epsilon=float('nan')), 'epsilon'), (lambda: layers.layer_norm_backward(x, x, None, torch.zeros(4, 2)), 'stats'),
+           (lambda: optim.orthogonalize([x, x.half()]), 'one element type'), (lambda: optim.orthogonalize(torch.zeros(1, 40000, device='cuda')), '40000')]
+  for f, text in cases:
+    with pytest.raises(ValueError, match=text):
+      f()
+  y = layers.dense(x.requires_grad_(True), w)
+  (g,) = torch.autograd.grad(y, x, torch.ones_like(y), create_graph=True)
+  with pytest.raises(RuntimeError):      # first order only
+    g.sum().backward()
+
+
+def test_c_refusals():
+  lib = N.load()
+  EINVAL, EDEVICE = -22, -5
+  buf = (C.c_float * 1024)()
+  p = (C.addressof(buf) + 255) // 256 * 256      # never reached: every call below is refused on the host
+
+  def fwd(**kw):
+    a = N.DenseForwardArgs(0, 0, 4, 4, 4, p, 4, p, 4, None, None, 0, p, 4, None)
+    for k, v in kw.items():
+      setattr(a, k, v)
+    return lib.nerfds_dense_forward(0, C.byref(a), None)
+
+  def bwd(**kw):
+    a = N.DenseBackwardArgs(0, 0, 4, 4, 4, p, 4, p, 4, p, 4, None, p, 4, p, p, p, 1 << 20)
+    for k, v in kw.items():
+      setattr(a, k, v)
+    return lib.nerfds_dense_backward(0, C.byref(a), None)
+
+  def nfwd(**kw):
+    a = N.LayerNormForwardArgs(0, 4, 4, 1e-6, p, 4, None, None, p, 4, None)
+    for k, v in kw.items():
+      setattr(a, k, v)
+    return lib.nerfds_layer_norm_forward(0, C.byref(a), None)
+
+  def nbwd(**kw):
+    a = N.LayerNormBackwardArgs(0, 4, 4, p, 4, None, p, 4, p, p, 4, p, p, p, 1 << 20)
+    for k, v in kw.items():
+      setattr(a, k, v)
+    return lib.nerfds_layer_norm_backward(0, C.byref(a), None)
+
+  bad = [dict(dtype=3), dict(dtype=-1), dict(m=-1), dict(m=1 << 41), dict(x=None), dict(x=p + 1), dict(ldx=3)]
+  for kw in bad + [dict(activation=6), dict(k=0), dict(n=0), dict(kernel=None), dict(ldk=3), dict(y=None), dict(ldy=2), dict(bias=p + 2), dict(residual=p, ldr=3),
+                   dict(m=1 << 40, n=1 << 20), dict(activation=2, save=p + 2)]:
+    assert fwd(**kw) == EINVAL, kw
+    assert b'nerfds_dense_forward' in lib.nerfds_last_error(None)
+  for kw in bad + [dict(activation=-1), dict(n=0), dict(dy=None), dict(lddy=3), dict(lddx=1), dict(activation=1), dict(dkernel=p + 1)]:
+    assert bwd(**kw) == EINVAL, kw
+  for kw in bad + [dict(d=0), dict(epsilon=-1.0), dict(epsilon=float('inf')), dict(epsilon=float('nan')), dict(y=None), dict(ldy=1), dict(scale=p + 3)]:
+    assert nfwd(**kw) == EINVAL, kw
+  for kw in bad + [dict(d=-4), dict(dy=None), dict(stats=None), dict(lddx=1), dict(dbias=p + 1)]:
+    assert nbwd(**kw) == EINVAL, kw
+  for f in (lib.nerfds_dense_forward, lib.nerfds_dense_backward, lib.nerfds_layer_norm_forward, lib.nerfds_layer_norm_backward):
+    assert f(0, None, None) == EINVAL
+  assert fwd(m=0, x=None) == 0 and nfwd(m=0, y=None) == 0
+
+  def ortho(dtype=0, count=1, steps=5, ws=p, nbytes=1 << 20, **kw):
+    mat = N.Matrix(p, 4, p, 4, 4, 4)
+    for k, v in kw.items():
+      setattr(mat, k, v)
+    return lib.nerfds_orthogonalize(0, dtype, C.byref(mat), count, steps, ws, nbytes, None)
+  for kw in (dict(dtype=9), dict(count=-1), dict(steps=0), dict(steps=17), dict(ws=None), dict(ws=p + 8), dict(nbytes=16), dict(rows=0), dict(cols=-1), dict(rows=40000), dict(u=None),
+             dict(ldu=3), dict(ldo=3), dict(o=p + 1)):
+    assert ortho(**kw) == EINVAL, kw
+  assert ortho(count=0) == 0 and lib.nerfds_orthogonalize(0, 0, None, 1, 5, p, 1 << 20, None) == EINVAL
+  assert lib.nerfds_dense_save_bytes(1, 1, 5, 9) == 10 and lib.nerfds_dense_save_bytes(0, 5, 5, 9) == 180 and lib.nerfds_dense_save_bytes(2, 0, 5, 9) == 0
+  assert lib.nerfds_dense_save_bytes(2, 7, 5, 9) == EINVAL
+  a = N.DenseForwardArgs(0, 0, 4, 4, 4, p, 4, p, 4, None, None, 0, p, 4, None)
+  assert lib.nerfds_dense_forward(1000, C.byref(a), None) == EDEVICE and lib.nerfds_dense_forward(-1, C.byref(a), None) == EDEVICE
+
+
+def test_struct_sizes_of_the_operators():
+  lib = N.load()
+  for which, st in ((9, N.DenseForwardArgs), (10, N.DenseBackwardArgs), (11, N.LayerNormForwardArgs), (12, N.LayerNormBackwardArgs), (13, N.Matrix)):
+    assert lib.nerfds_struct_size(which) == C.sizeof(st)
