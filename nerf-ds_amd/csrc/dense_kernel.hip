@@ -7,6 +7,9 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
+#include "lds_attr.h"
 #include "operators.h"
 #include "operators_dev.h"
 
@@ -135,28 +138,83 @@ template <typename T, bool CONT> struct Tile {
   }
 };
 
-OPS_DEV float sigmoid_(float z) { return 1.f / (1.f + expf(-z)); }
-OPS_DEV float act_value(float z, int act) {
-  switch (act) {
-    case ACT_RELU: return z > 0.f || z != z ? z : 0.f;
-    case ACT_SIGMOID: return sigmoid_(z);
-    case ACT_SOFTPLUS: return fmaxf(z, 0.f) + log1pf(expf(-fabsf(z)));
-    case ACT_SILU: return z * sigmoid_(z);
-    case ACT_GELU: return 0.5f * z * erfcf(-0.70710678f * z);      // (erfc: 1 + erf cancels for negative z)
-    default: return z;
+// Activations.  For 16-bit results exp and 1 / x are the hardware's instructions (1 ulp of float32, 2^-12 of what the result keeps), log1p a series where e is
+// small, and erfc(x) = t (a1 + t (a2 + ...)) exp(-x^2), t = 1 / (1 + p x), Abramowitz & Stegun 7.1.26 (absolute error 1.5e-7): the library's erfcf is 100
+// instructions, 85 us of 33 million outputs.  float32 results take the library's functions.
+template <typename T> OPS_DEV float exp_(float x) {
+  if constexpr (sizeof(T) == 4) return expf(x); else return __builtin_amdgcn_exp2f(x * 1.44269504f);
+}
+template <typename T> OPS_DEV float sigmoid_(float z) {
+  if constexpr (sizeof(T) == 4) return 1.f / (1.f + expf(-z)); else return __builtin_amdgcn_rcpf(1.f + exp_<T>(-z));
+}
+template <typename T> OPS_DEV float log1p_exp_(float z) {      // log(1 + exp(z)), z <= 0
+  const float e = exp_<T>(z);
+  if constexpr (sizeof(T) == 4) return log1pf(e);
+  else return e < 0.01f ? e * (1.f - e * (0.5f - e * 0.33333333f)) : 0.69314718f * __builtin_amdgcn_logf(1.f + e);      // (v_log_f32: base 2)
+}
+template <typename T> OPS_DEV float cdf_(float z) {            // of the normal distribution
+  if constexpr (sizeof(T) == 4) return 0.5f * erfcf(-0.70710678f * z);      // (erfc: 1 + erf cancels for negative z)
+  else {
+    const float x = 0.70710678f * fabsf(z), t = __builtin_amdgcn_rcpf(1.f + 0.3275911f * x);
+    const float q = 0.5f * t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f)))) * exp_<T>(-x * x);
+    return z < 0.f ? q : 1.f - q;
   }
 }
-OPS_DEV float act_slope(float z, int act) {
+template <typename T, int ACT> OPS_DEV float act_value(float z) {
+  if constexpr (ACT == ACT_RELU) return z > 0.f || z != z ? z : 0.f;
+  if constexpr (ACT == ACT_SIGMOID) return sigmoid_<T>(z);
+  if constexpr (ACT == ACT_SOFTPLUS) return fmaxf(z, 0.f) + log1p_exp_<T>(-fabsf(z));
+  if constexpr (ACT == ACT_SILU) return z * sigmoid_<T>(z);
+  if constexpr (ACT == ACT_GELU) return z * cdf_<T>(z);
+  return z;
+}
+template <typename T, int ACT> OPS_DEV float act_slope(float z) {
+  if constexpr (ACT == ACT_SIGMOID) { const float s = sigmoid_<T>(z); return s * (1.f - s); }
+  if constexpr (ACT == ACT_SOFTPLUS) return sigmoid_<T>(z);
+  if constexpr (ACT == ACT_SILU) { const float s = sigmoid_<T>(z); return s * (1.f + z * (1.f - s)); }
+  if constexpr (ACT == ACT_GELU) return cdf_<T>(z) + z * exp_<T>(-0.5f * z * z) * 0.39894228f;
+  return 1.f;
+}
+// The switch stands around 8 elements, and the loops that come here are not unrolled: a copy of every activation for every element of a tile is
+// 150 KB of code that a wave jumps through, and the tile then waits for its instructions (382 us instead of 250 for 524288 x 256 x 256).
+template <typename T> OPS_DEV void act_values(float (&v)[8], int act) {
   switch (act) {
-    case ACT_SIGMOID: { const float s = sigmoid_(z); return s * (1.f - s); }
-    case ACT_SOFTPLUS: return sigmoid_(z);
-    case ACT_SILU: { const float s = sigmoid_(z); return s * (1.f + z * (1.f - s)); }
-    case ACT_GELU: return 0.5f * erfcf(-0.70710678f * z) + z * expf(-0.5f * z * z) * 0.39894228f;
-    default: return 1.f;
+#define CASE(A) case A: _Pragma("unroll") for (int j = 0; j < 8; ++j) v[j] = act_value<T, A>(v[j]); break;
+    CASE(ACT_RELU) CASE(ACT_SIGMOID) CASE(ACT_SOFTPLUS) CASE(ACT_SILU) CASE(ACT_GELU)
+#undef CASE
+    default: break;
+  }
+}
+template <typename T> OPS_DEV void act_slopes(float (&v)[8], int act) {
+  switch (act) {
+#define CASE(A) case A: _Pragma("unroll") for (int j = 0; j < 8; ++j) v[j] = act_slope<T, A>(v[j]); break;
+    CASE(ACT_SIGMOID) CASE(ACT_SOFTPLUS) CASE(ACT_SILU) CASE(ACT_GELU)
+#undef CASE
+    default: break;
   }
 }
 
-enum { OUT_FORWARD = 0, OUT_PLAIN = 1, OUT_PARTIAL = 2 };
+// The end of the forward for 8 elements of row m, columns n ..: what the backward needs, activation, residual, the one rounding
+template <typename T> OPS_DEV void finish(float (&v)[8], long long m, long long n, long long valid, int act, void* save, long long lds, const void* residual, long long ldr, void* y,
+                                          long long ldy) {
+  if (save != nullptr) {
+    if (act == ACT_RELU) {
+      unsigned bits = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) bits |= (v[j] > 0.f ? 1u : 0u) << j;
+      static_cast<unsigned char*>(save)[m * lds + (n >> 3)] = (unsigned char)bits;
+    } else if (act != ACT_NONE) gran_store<T>(static_cast<T*>(save) + m * lds + n, gran_pack<T>(v), valid);
+  }
+  act_values<T>(v, act);
+  if (residual != nullptr) {
+    const Gran<T> g = gran_load<T>(static_cast<const T*>(residual) + m * ldr + n, valid);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] += gran_get<T>(g, j);
+  }
+  gran_store<T>(static_cast<T*>(y) + m * ldy + n, gran_pack<T>(v), valid);
+}
+
+enum { OUT_FORWARD = 0, OUT_PLAIN = 1, OUT_WEIGHTS = 2 };      // weights: partial sums of a split (part), or the result (y) where one split does it
 
 template <typename T, bool AC, bool BC, int OUT, int MASK /* 0, or the operand (1 = a, 2 = b) the relu bits belong to */>
 __global__ __launch_bounds__(THREADS, 2) void k_gemm(const GemmArgs G) {
@@ -173,7 +231,7 @@ __global__ __launch_bounds__(THREADS, 2) void k_gemm(const GemmArgs G) {
   f32x16 acc[2][2] = {};
   Gran<T> ra[TA::NG], rb[TB::NG];
   float cs[8] = {};
-  const bool sums = OUT == OUT_PARTIAL && G.colpart != nullptr && m0 == 0;
+  const bool sums = OUT == OUT_WEIGHTS && G.colpart != nullptr && m0 == 0;
   auto fetch = [&](long long c) __attribute__((always_inline)) {
     TA::load(ra, G.a, G.lda, m0, G.M, c, c1);
     TB::load(rb, G.b, G.ldb, n0, G.N, c, c1);
@@ -185,7 +243,7 @@ __global__ __launch_bounds__(THREADS, 2) void k_gemm(const GemmArgs G) {
     __syncthreads();
     TA::stage(ra, lds);
     TB::stage(rb, lds + TA::BYTES);
-    if constexpr (OUT == OUT_PARTIAL) {
+    if constexpr (OUT == OUT_WEIGHTS) {
       if (sums) {
 #pragma unroll
         for (int i = 0; i < TB::NG; ++i)
@@ -218,9 +276,9 @@ __global__ __launch_bounds__(THREADS, 2) void k_gemm(const GemmArgs G) {
     }
   }
 
-  if constexpr (OUT == OUT_PARTIAL) {
+  if constexpr (OUT == OUT_WEIGHTS) {
     if (G.part != nullptr) {
-      float* out = G.part + (size_t)blockIdx.y * G.M * G.N;
+      float* out = G.part + blockIdx.y * ((G.M * G.N + 3) & ~3LL);
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -242,10 +300,11 @@ __global__ __launch_bounds__(THREADS, 2) void k_gemm(const GemmArgs G) {
       if (threadIdx.x < 128 && n0 + threadIdx.x < G.N) {
         float s = 0.f;
         for (int q = 0; q < 16; ++q) s += red[q * 128 + threadIdx.x];
-        G.colpart[(size_t)blockIdx.y * G.N + n0 + threadIdx.x] = s;
+        G.colpart[blockIdx.y * ((G.N + 3) & ~3LL) + n0 + threadIdx.x] = s;
       }
     }
-  } else {
+  }
+  if (OUT != OUT_WEIGHTS || G.y != nullptr) {
     // the wave's 64 x 64 block through LDS, 32 rows at a time, so that every lane finishes 8 consecutive elements of a row
     float* buf = reinterpret_cast<float*>(lds) + wave * 32 * 68;
     const long long n = n0 + 64 * wn + 8 * (lane & 7), valid = G.N - n;
@@ -263,7 +322,7 @@ __global__ __launch_bounds__(THREADS, 2) void k_gemm(const GemmArgs G) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) buf[((r & 3) + 8 * (r >> 2) + 4 * (lane >> 5)) * 68 + 32 * j + (lane & 31)] = acc[i][j][r];
       __syncthreads();
-#pragma unroll
+#pragma unroll 1
       for (int q = 0; q < 4; ++q) {
         const int row = 8 * q + (lane >> 3);
         const long long m = m0 + 64 * wm + 32 * i + row;
@@ -274,36 +333,59 @@ __global__ __launch_bounds__(THREADS, 2) void k_gemm(const GemmArgs G) {
         if constexpr (OUT == OUT_FORWARD) {
 #pragma unroll
           for (int j = 0; j < 8; ++j) v[j] += bias[j];
-          if (G.act == ACT_RELU) {
-            unsigned bits = 0;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) bits |= (v[j] > 0.f ? 1u : 0u) << j;
-            if (G.save != nullptr) static_cast<unsigned char*>(G.save)[m * G.lds + (n >> 3)] = (unsigned char)bits;
-          } else if (G.act != ACT_NONE && G.save != nullptr)
-            gran_store<T>(static_cast<T*>(G.save) + m * G.lds + n, gran_pack<T>(v), valid);
-          if (G.act != ACT_NONE) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = act_value(v[j], G.act);
-          }
-          if (G.residual != nullptr) {
-            const Gran<T> g = gran_load<T>(static_cast<const T*>(G.residual) + m * G.ldr + n, valid);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] += gran_get<T>(g, j);
-          }
-        }
-        gran_store<T>(static_cast<T*>(G.y) + m * G.ldy + n, gran_pack<T>(v), valid);
+          finish<T>(v, m, n, valid, G.act, G.save, G.lds, G.residual, G.ldr, G.y, G.ldy);
+        } else gran_store<T>(static_cast<T*>(G.y) + m * G.ldy + n, gran_pack<T>(v), valid);
       }
     }
   }
 }
 
-// out[i] = sum over the splits, rounded once
-template <typename T> __global__ __launch_bounds__(256) void k_sum_splits(const float* __restrict__ part, int splits, long long count, T* __restrict__ out) {
-  const long long i = blockIdx.x * 256LL + threadIdx.x;
-  if (i >= count) return;
-  float s = 0.f;
-  for (int q = 0; q < splits; ++q) s += part[q * count + i];
-  out[i] = from_f32<T>(s);
+#include "dense_tile.h"
+#include "dense_resident.h"
+
+// The forward of a few rows (m <= 8: one frame's embedding, one token): bound by reading the kernel once, so by how many loads are in flight.  A workgroup
+// takes 32 columns - a cache line's worth of every kernel row - and all of k: thread (slice, granule) multiplies 8 rows of 8 columns at a time, and
+// the 64 slices are added over shuffles and LDS.  float32 multiply-adds: the matrix pipe would run 32-row tiles with 31 of them empty
+// (1 x 1024 x 1024 bf16: 4.5 us against 29 us through the tile kernel, whose 16 steps each wait for memory).
+template <typename T, int M> __global__ __launch_bounds__(256) void k_rows(const DenseFwd A) {
+  __shared__ float red[4][M][32];
+  const int g = threadIdx.x & 3, slice = threadIdx.x >> 2;
+  const long long n = blockIdx.x * 32LL + 8 * g, valid = A.n - n;
+  float acc[M][8] = {};
+  for (int k = slice * 8; k < A.k; k += 512) {
+    Gran<T> x[M], w[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) w[r] = gran_load<T>(static_cast<const T*>(A.kernel) + (k + r) * A.ldk + n, k + r < A.k ? valid : 0);
+#pragma unroll
+    for (int m = 0; m < M; ++m) x[m] = gran_load<T>(static_cast<const T*>(A.x) + m * A.ldx + k, m < A.m ? A.k - k : 0);
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int m = 0; m < M; ++m) acc[m][j] = fmaf(gran_get<T>(x[m], r), gran_get<T>(w[r], j), acc[m][j]);
+  }
+#pragma unroll
+  for (int m = 0; m < M; ++m)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      float v = acc[m][j];
+#pragma unroll
+      for (int d = 4; d < 64; d <<= 1) v += __shfl_xor(v, d, 64);
+      if ((threadIdx.x & 63) < 4) red[threadIdx.x >> 6][m][8 * g + j] = v;
+    }
+  __syncthreads();
+  const int m = threadIdx.x >> 2;
+  if (m >= M || m >= A.m || valid <= 0) return;
+  float v[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = red[0][m][8 * g + j] + red[1][m][8 * g + j] + red[2][m][8 * g + j] + red[3][m][8 * g + j];
+  if (A.bias != nullptr) {
+    const Gran<T> b = gran_load<T>(static_cast<const T*>(A.bias) + n, valid);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] += gran_get<T>(b, j);
+  }
+  finish<T>(v, m, n, valid, A.act, A.save, A.act == ACT_RELU ? (A.n + 7) / 8 : A.n, A.residual, A.ldr, A.y, A.ldy);
 }
 
 // dz = dy act'(z), once, for the activations whose slope costs more than a bit test (the products below read dz once per tile of their other axis).
@@ -316,7 +398,10 @@ template <typename T> __global__ __launch_bounds__(256) void k_dz(const T* __res
     const Gran<T> a = gran_load<T>(dy + row * lddy + c, n - c), b = gran_load<T>(z + row * n + c, n - c);
     float v[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = gran_get<T>(a, j) * act_slope(gran_get<T>(b, j), act);
+    for (int j = 0; j < 8; ++j) v[j] = gran_get<T>(b, j);
+    act_slopes<T>(v, act);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] *= gran_get<T>(a, j);
     gran_store<T>(dz + row * n + c, gran_pack<T>(v), n - c);
   }
 }
@@ -324,30 +409,95 @@ template <typename T> __global__ __launch_bounds__(256) void k_dz(const T* __res
 long long up(long long a, long long b) { return (a + b - 1) / b; }
 size_t aligned(size_t b) { return (b + 255) & ~(size_t)255; }
 
-struct Splits { int count; long long cps; };
-// The weight gradient has few output tiles (4 for 256 x 256) and a long contraction: as many splits as give two workgroups per CU, none shorter than 4 steps
-Splits weight_splits(long long m, int k, int n, int bk, int num_cus) {
-  const long long tiles = up(k, BM) * up(n, BN), steps = up(m, bk);
-  long long want = up(2LL * num_cus, tiles);
-  if (want > up(steps, 4)) want = up(steps, 4);
-  if (want < 1) want = 1;
-  const long long cps = up(steps, want) * bk;
-  return {(int)up(m, cps), cps};
+bool whole_granules(const void* p, long long ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0; }
+// whether the weight gradient can go through k_tile: its operands' rows are whole, aligned granules, relu bits whole dwords (a smooth activation's dz is ours)
+bool weight_tiles_large(const DenseBwd& w) {
+  if (w.dtype == F32 || w.k % 8 || w.n % 8 || !whole_granules(w.x, w.ldx)) return false;
+  if (w.act == ACT_NONE || w.act == ACT_RELU) { if (!whole_granules(w.dy, w.lddy)) return false; }
+  return w.act != ACT_RELU || (w.n % 32 == 0 && reinterpret_cast<uintptr_t>(w.save) % 4 == 0);
 }
 
-template <typename T, bool AC, bool BC, int OUT, int MASK> void launch(hipStream_t st, GemmArgs& G) {
+struct Splits { int count; long long cps; };
+// The weight gradient has few output tiles (1 for 256 x 256) and a long contraction: as many splits as fill the card - one workgroup per CU of the large tiles,
+// two of the small ones -, none shorter than 256 rows.  A fraction of a round more is no gain: splits are rounded down there.
+Splits weight_splits(const DenseBwd& w, int num_cus) {
+  const bool large = weight_tiles_large(w);
+  const long long tiles = large ? up(w.k, 256) * up(w.n, w.n > 128 ? 256 : 128) : up(w.k, BM) * up(w.n, BN), slots = large ? num_cus : 2LL * num_cus, steps = up(w.m, 64);
+  long long want = tiles >= slots ? 1 : slots / tiles;
+  if (want > up(steps, 4)) want = up(steps, 4);
+  const long long cps = up(steps, want) * 64;
+  return {(int)up(w.m, cps), cps};
+}
+
+size_t weight_part_bytes(int splits, long long kn) { return splits > 1 ? aligned((size_t)splits * up(kn, 4) * 16) : 0; }      // (one split writes the result itself)
+
+// Whether k_tile can take the product: rows of whole, aligned granules on both sides (M, N and C too where they run along rows), relu bits in whole dwords
+template <bool AC, bool BC, int MASK> bool tile_fits(const GemmArgs& G) {
+  return whole_granules(G.a, G.lda) && whole_granules(G.b, G.ldb) && G.N % 8 == 0 && ((!AC && !BC) || G.C % 8 == 0) && (AC || G.M % 8 == 0) &&
+         (!MASK || (G.ldm % 4 == 0 && reinterpret_cast<uintptr_t>(G.mask) % 4 == 0));
+}
+template <typename T, typename GR, bool AC, bool BC, int OUT, int MASK, int ACT = ACT_NONE> void launch_tile(hipStream_t st, GemmArgs& G, int num_cus) {
+  if constexpr (OUT == OUT_FORWARD && ACT + 1 < ACT_COUNT) {
+    if (G.act != ACT) { launch_tile<T, GR, AC, BC, OUT, MASK, ACT + 1>(st, G, num_cus); return; }
+  }
+  auto kern = k_tile<T, GR, AC, BC, OUT, MASK, ACT>;
+  constexpr int lds = 4 * (GR::BM * 64 + GR::BN * 64 + (MASK ? 1024 : 0));
+  nerfds::allow_dynamic_lds(reinterpret_cast<const void*>(kern), lds);
+  G.tiles_n = (int)up(G.N, GR::BN);
+  G.tiles = up(G.M, GR::BM) * G.tiles_n;
+  const long long items = G.tiles * G.splits;
+  hipLaunchKernelGGL(kern, dim3((unsigned)(items < num_cus ? items : num_cus)), dim3(512), lds, st, G);
+}
+
+constexpr int LDS_BYTES = 160 * 1024, RESIDENT_N = 256, RESIDENT_M = 16384;
+template <typename T, bool BC, int NP, int OUT, bool MASK, int ACT = ACT_NONE> void launch_resident(hipStream_t st, GemmArgs& G, int num_cus) {
+  if constexpr (OUT == OUT_FORWARD && ACT + 1 < ACT_COUNT) {
+    if (G.act != ACT) { launch_resident<T, BC, NP, OUT, MASK, ACT + 1>(st, G, num_cus); return; }
+  }
+  auto kern = k_resident<T, BC, NP, OUT, MASK, ACT>;
+  nerfds::allow_dynamic_lds(reinterpret_cast<const void*>(kern), LDS_BYTES);
+  const long long want = up(G.M, 128);
+  hipLaunchKernelGGL(kern, dim3((unsigned)(want < num_cus ? want : num_cus)), dim3(512), Resident::bytes((int)G.N, (int)G.C + (G.bias != nullptr)), st, G);
+}
+
+template <typename T, bool AC, bool BC, int OUT, int MASK> void launch(hipStream_t st, GemmArgs& G, int num_cus) {
+  if constexpr (sizeof(T) == 2 && AC && OUT != OUT_WEIGHTS && MASK < 2) {
+    // Many rows past a kernel that fits LDS.  RESIDENT_M: every workgroup fills 128 KiB of LDS first (3 us), which wants some 100 rows behind it
+    if (G.M >= RESIDENT_M && G.N <= RESIDENT_N && G.C <= 4096 && Resident::bytes((int)G.N, (int)G.C + (G.bias != nullptr)) <= LDS_BYTES) {
+      if (G.N <= 64) launch_resident<T, BC, 2, OUT, MASK == 1>(st, G, num_cus);
+      else if (G.N <= 128) launch_resident<T, BC, 4, OUT, MASK == 1>(st, G, num_cus);
+      else launch_resident<T, BC, 8, OUT, MASK == 1>(st, G, num_cus);
+      return;
+    }
+  }
+  if constexpr (sizeof(T) == 2) {
+    // The large tiles pay where they fill the card; with fewer the 128 x 128 tiles below spread the work over more CUs
+    if (tile_fits<AC, BC, MASK>(G) && (OUT == OUT_WEIGHTS || up(G.M, 256) * up(G.N, 128) >= num_cus / 2)) {
+      if (G.N > 128) launch_tile<T, Grid256, AC, BC, OUT, MASK>(st, G, num_cus);
+      else launch_tile<T, Grid128, AC, BC, OUT, MASK>(st, G, num_cus);
+      return;
+    }
+  }
   G.tiles_n = (int)up(G.N, BN);
   G.tiles = up(G.M, BM) * G.tiles_n;
   hipLaunchKernelGGL((k_gemm<T, AC, BC, OUT, MASK>), dim3((unsigned)G.tiles, G.splits), dim3(THREADS), 0, st, G);
 }
 
-template <typename T> void forward_t(hipStream_t st, const DenseFwd& f) {
+template <typename T> void forward_t(hipStream_t st, const DenseFwd& f, int num_cus) {
+  if (f.m <= 8) {
+    const dim3 grid((unsigned)up(f.n, 32));
+    if (f.m == 1) hipLaunchKernelGGL((k_rows<T, 1>), grid, dim3(256), 0, st, f);
+    else if (f.m <= 2) hipLaunchKernelGGL((k_rows<T, 2>), grid, dim3(256), 0, st, f);
+    else if (f.m <= 4) hipLaunchKernelGGL((k_rows<T, 4>), grid, dim3(256), 0, st, f);
+    else hipLaunchKernelGGL((k_rows<T, 8>), grid, dim3(256), 0, st, f);
+    return;
+  }
   GemmArgs G{};
   G.a = f.x; G.lda = f.ldx; G.b = f.kernel; G.ldb = f.ldk; G.M = f.m; G.N = f.n; G.C = f.k;
   G.bias = f.bias; G.residual = f.residual; G.ldr = f.ldr; G.y = f.y; G.ldy = f.ldy; G.act = f.act;
   G.save = f.save; G.lds = f.act == ACT_RELU ? up(f.n, 8) : f.n;
   G.splits = 1; G.cps = f.k;
-  launch<T, true, false, OUT_FORWARD, 0>(st, G);
+  launch<T, true, false, OUT_FORWARD, 0>(st, G, num_cus);
 }
 
 template <typename T> void backward_t(hipStream_t st, const DenseBwd& w, int num_cus) {
@@ -366,22 +516,22 @@ template <typename T> void backward_t(hipStream_t st, const DenseBwd& w, int num
     GemmArgs G{};
     G.a = dz; G.lda = lddz; G.b = w.kernel; G.ldb = w.ldk; G.M = w.m; G.N = w.k; G.C = w.n;
     G.mask = bits; G.ldm = up(w.n, 8); G.y = w.dx; G.ldy = w.lddx; G.splits = 1; G.cps = w.n;
-    if (bits) launch<T, true, true, OUT_PLAIN, 1>(st, G); else launch<T, true, true, OUT_PLAIN, 0>(st, G);
+    if (bits) launch<T, true, true, OUT_PLAIN, 1>(st, G, num_cus); else launch<T, true, true, OUT_PLAIN, 0>(st, G, num_cus);
   }
   if (w.dkernel != nullptr || w.dbias != nullptr) {
-    const Splits s = weight_splits(w.m, w.k, w.n, Shape<T>::BK, num_cus);
+    const Splits s = weight_splits(w, num_cus);
     GemmArgs G{};
     G.a = w.x; G.lda = w.ldx; G.b = dz; G.ldb = lddz; G.N = w.n; G.C = w.m;
     G.M = w.dkernel ? w.k : 1;      // (the bias gradient alone: it rides on the first tile of the kernel's rows)
     G.mask = bits; G.ldm = up(w.n, 8); G.splits = s.count; G.cps = s.cps;
-    G.part = w.dkernel ? reinterpret_cast<float*>(ws) : nullptr;
-    float* col = reinterpret_cast<float*>(ws + aligned((size_t)s.count * w.k * w.n * 4));
+    const long long kn = (long long)w.k * w.n;
+    const size_t part_bytes = weight_part_bytes(s.count, kn);
+    G.part = w.dkernel && s.count > 1 ? reinterpret_cast<float*>(ws) : nullptr;
+    if (s.count == 1) { G.y = w.dkernel; G.ldy = w.n; }
+    float* col = reinterpret_cast<float*>(ws + part_bytes);
     G.colpart = w.dbias ? col : nullptr;
-    if (bits) launch<T, false, false, OUT_PARTIAL, 2>(st, G); else launch<T, false, false, OUT_PARTIAL, 0>(st, G);
-    if (w.dkernel)
-      hipLaunchKernelGGL((k_sum_splits<T>), dim3((unsigned)up((long long)w.k * w.n, 256)), dim3(256), 0, st, G.part, s.count, (long long)w.k * w.n, static_cast<T*>(w.dkernel));
-    if (w.dbias)
-      hipLaunchKernelGGL((k_sum_splits<T>), dim3((unsigned)up(w.n, 256)), dim3(256), 0, st, col, s.count, (long long)w.n, static_cast<T*>(w.dbias));
+    if (bits) launch<T, false, false, OUT_WEIGHTS, 2>(st, G, num_cus); else launch<T, false, false, OUT_WEIGHTS, 0>(st, G, num_cus);
+    sum_splits<T>(st, SplitSum{G.part, up(kn, 4) * 4, kn, G.part ? w.dkernel : nullptr}, SplitSum{col, up(w.n, 4) * 4, w.n, w.dbias}, s.count);
   }
 }
 
@@ -391,24 +541,20 @@ size_t dense_save_bytes(int dtype, int act, long long m, int n) {
   return act == ACT_NONE ? 0 : act == ACT_RELU ? (size_t)m * up(n, 8) : (size_t)m * n * dtype_bytes(dtype);
 }
 size_t dense_bwd_ws(const DenseBwd& a, int num_cus) {
-  const Splits s = weight_splits(a.m, a.k, a.n, a.dtype == F32 ? Shape<float>::BK : Shape<f16_t>::BK, num_cus);
+  const Splits s = weight_splits(a, num_cus);
   size_t b = a.act != ACT_NONE && a.act != ACT_RELU ? aligned((size_t)a.m * a.n * dtype_bytes(a.dtype)) : 0;
-  if (a.dkernel != nullptr || a.dbias != nullptr) b += aligned((size_t)s.count * a.k * a.n * 4) + aligned((size_t)s.count * a.n * 4);
+  if (a.dkernel != nullptr || a.dbias != nullptr) b += weight_part_bytes(s.count, (long long)a.k * a.n) + aligned((size_t)s.count * up(a.n, 4) * 16);
   return b;
 }
-void dense_forward(hipStream_t st, const DenseFwd& a, int) {
-  if (a.dtype == F32) forward_t<float>(st, a);
-  else if (a.dtype == F16) forward_t<f16_t>(st, a);
-  else forward_t<bf16_t>(st, a);
+void dense_forward(hipStream_t st, const DenseFwd& a, int num_cus) {
+  if (a.dtype == F32) forward_t<float>(st, a, num_cus);
+  else if (a.dtype == F16) forward_t<f16_t>(st, a, num_cus);
+  else forward_t<bf16_t>(st, a, num_cus);
 }
 void dense_backward(hipStream_t st, const DenseBwd& a, int num_cus) {
   if (a.m == 0) {      // an empty sum is zero
     const long long kn = (long long)a.k * a.n;
-#define CLEAR(T)                                                                                                                                                  \
-    do {                                                                                                                                                          \
-      if (a.dkernel) hipLaunchKernelGGL((k_sum_splits<T>), dim3((unsigned)up(kn, 256)), dim3(256), 0, st, nullptr, 0, kn, static_cast<T*>(a.dkernel));           \
-      if (a.dbias) hipLaunchKernelGGL((k_sum_splits<T>), dim3((unsigned)up(a.n, 256)), dim3(256), 0, st, nullptr, 0, (long long)a.n, static_cast<T*>(a.dbias));  \
-    } while (0)
+#define CLEAR(T) sum_splits<T>(st, SplitSum{nullptr, 0, kn, a.dkernel}, SplitSum{nullptr, 0, a.n, a.dbias}, 0)
     if (a.dtype == F32) CLEAR(float); else if (a.dtype == F16) CLEAR(f16_t); else CLEAR(bf16_t);
 #undef CLEAR
     return;

@@ -82,7 +82,7 @@ __global__ __launch_bounds__(THREADS) void k_norm_fwd(const NormFwd A) {
   }
 }
 
-// part: [grid][2][d] - column sums of dy xh, of dy
+// part: [grid][2][d rounded up to 4] - column sums of dy xh, of dy
 template <typename T, int LPR, int NG>
 __global__ __launch_bounds__(THREADS) void k_norm_bwd(const NormBwd A, float* __restrict__ part) {
   constexpr int ROWS = THREADS / LPR;
@@ -133,7 +133,8 @@ __global__ __launch_bounds__(THREADS) void k_norm_bwd(const NormBwd A, float* __
     }
   }
   if (part == nullptr) return;
-  float* out = part + (size_t)blockIdx.x * 2 * d;
+  const int dp = (d + 3) & ~3;
+  float* out = part + (size_t)blockIdx.x * 2 * dp;
 #pragma unroll
   for (int k = 0; k < 2; ++k)
 #pragma unroll
@@ -141,7 +142,7 @@ __global__ __launch_bounds__(THREADS) void k_norm_bwd(const NormBwd A, float* __
       if constexpr (LPR == THREADS) {
         const int c = 8 * (l + g * LPR);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) if (c + j < d) out[k * d + c + j] = k == 0 ? ds[g][j] : db[g][j];
+        for (int j = 0; j < 8; ++j) if (c + j < d) out[k * dp + c + j] = k == 0 ? ds[g][j] : db[g][j];
       } else {      // the rows side by side in this workgroup: added through LDS, in the order of their number
         __syncthreads();
 #pragma unroll
@@ -151,7 +152,7 @@ __global__ __launch_bounds__(THREADS) void k_norm_bwd(const NormBwd A, float* __
           float s = 0.f;
           for (int r = 0; r < ROWS; ++r) s += cols[r * LPR * 8 + e];
           const int c = 8 * g * LPR + e;
-          if (c < d) out[k * d + c] = s;
+          if (c < d) out[k * dp + c] = s;
         }
       }
     }
@@ -181,10 +182,10 @@ template <typename T> __global__ __launch_bounds__(THREADS) void k_norm_fwd_long
 // (the column sums of a workgroup accumulate in its own partial: thread t owns the columns t + 256 i)
 template <typename T> __global__ __launch_bounds__(THREADS) void k_norm_bwd_long(const NormBwd A, float* __restrict__ part) {
   __shared__ float red[4];
-  const int d = A.d;
-  float* out = part + (size_t)blockIdx.x * 2 * d;
+  const int d = A.d, dp = (d + 3) & ~3;
+  float* out = part + (size_t)blockIdx.x * 2 * dp;
   if (part != nullptr)
-    for (int c = threadIdx.x; c < d; c += THREADS) { out[c] = 0.f; out[d + c] = 0.f; }
+    for (int c = threadIdx.x; c < d; c += THREADS) { out[c] = 0.f; out[dp + c] = 0.f; }
   for (long long row = blockIdx.x; row < A.m; row += gridDim.x) {
     const T* x = static_cast<const T*>(A.x) + row * A.ldx;
     const T* gy = static_cast<const T*>(A.dy) + row * A.lddy;
@@ -192,7 +193,7 @@ template <typename T> __global__ __launch_bounds__(THREADS) void k_norm_bwd_long
     float s1 = 0.f, s2 = 0.f;
     for (int c = threadIdx.x; c < d; c += THREADS) {
       const float dy = to_f32<T>(gy[c]), xh = (to_f32<T>(x[c]) - mu) * rstd, h = A.scale != nullptr ? dy * to_f32<T>(static_cast<const T*>(A.scale)[c]) : dy;
-      if (part != nullptr) { out[c] += dy * xh; out[d + c] += dy; }
+      if (part != nullptr) { out[c] += dy * xh; out[dp + c] += dy; }
       s1 += h;
       s2 += h * xh;
     }
@@ -205,23 +206,8 @@ template <typename T> __global__ __launch_bounds__(THREADS) void k_norm_bwd_long
   }
 }
 
-// dscale / dbias = sum of the workgroups' partials: 64 columns per workgroup, 4 threads deep per column
-template <typename T> __global__ __launch_bounds__(THREADS) void k_norm_sum(const float* __restrict__ part, int parts, int d, T* __restrict__ dscale, T* __restrict__ dbias) {
-  __shared__ float red[THREADS];
-  const int c = blockIdx.x * 64 + (threadIdx.x & 63), k = blockIdx.y;      // k: 0 dscale, 1 dbias
-  float s = 0.f;
-  if (c < d)
-    for (int p = threadIdx.x >> 6; p < parts; p += 4) s += part[((size_t)p * 2 + k) * d + c];
-  red[threadIdx.x] = s;
-  __syncthreads();
-  if (threadIdx.x < 64 && c < d) {
-    s = red[threadIdx.x] + red[threadIdx.x + 64] + red[threadIdx.x + 128] + red[threadIdx.x + 192];
-    T* out = k == 0 ? dscale : dbias;
-    if (out != nullptr) out[c] = from_f32<T>(s);
-  }
-}
-
 long long up(long long a, long long b) { return (a + b - 1) / b; }
+long long up4(long long a) { return (a + 3) & ~3LL; }
 
 // lanes per row and granules per lane: the fewest lanes that hold a row in 2 granules each, then whole waves of 4, then the workgroup; 0 = longer than that
 struct RowShape { int lpr, ng; };
@@ -255,7 +241,7 @@ template <typename T> void fwd_t(hipStream_t st, const NormFwd& a, int num_cus) 
 }
 template <typename T> void bwd_t(hipStream_t st, const NormBwd& a, int num_cus) {
   if (a.m == 0) {      // an empty sum is zero
-    hipLaunchKernelGGL((k_norm_sum<T>), dim3((unsigned)up(a.d, 64), 2), dim3(THREADS), 0, st, nullptr, 0, a.d, static_cast<T*>(a.dscale), static_cast<T*>(a.dbias));
+    sum_splits<T>(st, SplitSum{nullptr, 0, a.d, a.dscale}, SplitSum{nullptr, 0, a.d, a.dbias}, 0);
     return;
   }
   const RowShape s = row_shape(a.d);
@@ -266,14 +252,13 @@ template <typename T> void bwd_t(hipStream_t st, const NormBwd& a, int num_cus) 
   NORM_SHAPES(X)
 #undef X
   if (!done) hipLaunchKernelGGL((k_norm_bwd_long<T>), dim3(grid), dim3(THREADS), 0, st, a, part);
-  if (part != nullptr)
-    hipLaunchKernelGGL((k_norm_sum<T>), dim3((unsigned)up(a.d, 64), 2), dim3(THREADS), 0, st, part, grid, a.d, static_cast<T*>(a.dscale), static_cast<T*>(a.dbias));
+  if (part != nullptr) sum_splits<T>(st, SplitSum{part, 2 * up4(a.d), a.d, a.dscale}, SplitSum{part + up4(a.d), 2 * up4(a.d), a.d, a.dbias}, grid);
 }
 
 }  // namespace
 
 size_t norm_bwd_ws(const NormBwd& a, int num_cus) {
-  return a.dscale != nullptr || a.dbias != nullptr ? (size_t)bwd_grid(a.m, a.d, num_cus) * 2 * a.d * sizeof(float) : 0;
+  return a.dscale != nullptr || a.dbias != nullptr ? (size_t)bwd_grid(a.m, a.d, num_cus) * 2 * up4(a.d) * sizeof(float) : 0;
 }
 void norm_forward(hipStream_t st, const NormFwd& a, int num_cus) {
   if (a.dtype == F32) fwd_t<float>(st, a, num_cus);

@@ -93,4 +93,44 @@ OPS_DEV long long xcd_order(long long wg, long long total) {
   return x * per + (x < rest ? x : rest) + i;
 }
 
+// ---- the second stage of a split sum --------------------------------------------------------------------------------------------------------
+// out[c] = sum over p of part[p stride + c], rounded once, for two sums (strides are multiples of 4: what lies between count and stride is read, not used)
+// in one launch (a weight's gradient and a bias's).  A lane takes 4 columns; DEEP threads share them, each adding every DEEP-th partial, and their sums are
+// added in their order: 16 where there are that many partials (one thread per column: 31 us for 128 partials of 256 x 256, so: 7 us), 1 below (2 partials of
+// 2048 x 4096: 50 us with 14 of 16 threads idle, 19 us).
+struct SplitSum { const float* part; long long stride, count; void* out; };
+template <typename T, int DEEP> __global__ __launch_bounds__(256) void k_sum_splits(SplitSum a, SplitSum b, int parts, unsigned blocks_a) {
+  constexpr int WIDE = 256 / DEEP;      // lanes along the columns
+  __shared__ f32x4 red[DEEP][WIDE];
+  const SplitSum S = blockIdx.x < blocks_a ? a : b;
+  const int l = threadIdx.x % WIDE, deep = threadIdx.x / WIDE;
+  const long long c0 = (long long)(blockIdx.x < blocks_a ? blockIdx.x : blockIdx.x - blocks_a) * (4 * WIDE), c = c0 + 4 * l;
+  f32x4 s = {0.f, 0.f, 0.f, 0.f};
+  if (c < S.count) {
+#pragma unroll 8
+    for (int p = deep; p < parts; p += DEEP) s += *reinterpret_cast<const f32x4*>(S.part + p * S.stride + c);
+  }
+  T* out = static_cast<T*>(S.out);
+  if constexpr (DEEP == 1) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) if (c + j < S.count) out[c + j] = from_f32<T>(s[j]);
+  } else {
+    red[deep][l] = s;
+    __syncthreads();
+    if (threadIdx.x < 4 * WIDE && c0 + threadIdx.x < S.count) {
+      float v = 0.f;
+      for (int q = 0; q < DEEP; ++q) v += red[q][threadIdx.x >> 2][threadIdx.x & 3];
+      out[c0 + threadIdx.x] = from_f32<T>(v);
+    }
+  }
+}
+template <typename T, int DEEP> void sum_splits_deep(hipStream_t st, SplitSum a, SplitSum b, int parts) {
+  const long long per = 1024 / DEEP;
+  const unsigned na = a.out ? (unsigned)((a.count + per - 1) / per) : 0, nb = b.out ? (unsigned)((b.count + per - 1) / per) : 0;
+  if (na + nb) hipLaunchKernelGGL((k_sum_splits<T, DEEP>), dim3(na + nb), dim3(256), 0, st, a, b, parts, na);
+}
+template <typename T> void sum_splits(hipStream_t st, SplitSum a, SplitSum b, int parts) {      // out == nullptr: that sum is not wanted
+  if (parts >= 16) sum_splits_deep<T, 16>(st, a, b, parts); else sum_splits_deep<T, 1>(st, a, b, parts);
+}
+
 }  // namespace nerfds_ops

@@ -129,13 +129,18 @@ class Out(C.Structure):
 ACTIVATIONS = {'none': 0, 'relu': 1, 'sigmoid': 2, 'softplus': 3, 'silu': 4, 'gelu': 5}
 
 
+_DTYPES = {'torch.float32': 0, 'torch.float16': 1, 'torch.bfloat16': 2}
+_dtype_codes = {}      # torch dtype -> code, filled on use (this module does not import torch)
+
+
 def dtype_code(dtype) -> int:
   """NERFDS_DTYPE_* of a torch dtype."""
-  import torch
-  codes = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-  if dtype not in codes:
-    raise ValueError(f'element type {dtype}: float32, float16 and bfloat16 are built')
-  return codes[dtype]
+  code = _dtype_codes.get(dtype)
+  if code is None:
+    if str(dtype) not in _DTYPES:
+      raise ValueError(f'element type {dtype}: float32, float16 and bfloat16 are built')
+    code = _dtype_codes[dtype] = _DTYPES[str(dtype)]
+  return code
 
 
 class DenseForwardArgs(C.Structure):

@@ -33,6 +33,8 @@ def _check_operands(what: str, x: torch.Tensor, **others) -> None:
 
 def _rows(t: torch.Tensor, cols: int, one_row: bool = False) -> Tuple[torch.Tensor, int]:
   """``t`` as [rows, cols] with unit stride along the columns, and its row stride (``one_row``: 0, one row for all, is allowed)."""
+  if t.is_contiguous():
+    return t, cols
   t = t.reshape(-1, cols)
   ld = t.stride(0) if t.shape[0] > 1 else cols
   if (cols > 1 and t.stride(1) != 1) or (ld < cols and not (one_row and ld == 0)):
@@ -44,16 +46,26 @@ def _ptr(t: Optional[torch.Tensor]):
   return t.data_ptr() if t is not None else None
 
 
+# the handle of torch's current stream of a device, without building a Stream object around it (the launch of a small layer costs less than that)
+_raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _call(what: str, fn, x: torch.Tensor, args) -> None:
-  rc = fn(x.device.index, C.byref(args), torch.cuda.current_stream(x.device).cuda_stream)
+  index = x.device.index
+  rc = fn(index, C.byref(args), _raw_stream(index))
   if rc != 0:
     raise RuntimeError(f'{what} failed ({rc}): {N.last_error(None)}')
 
 
-def _workspace(nbytes: int, x: torch.Tensor) -> Optional[torch.Tensor]:
+def _call_with_workspace(what: str, query, fn, x: torch.Tensor, args) -> None:
+  index = x.device.index
+  nbytes = query(index, C.byref(args))
   if nbytes < 0:
-    raise RuntimeError(f'workspace query failed ({nbytes}): {N.last_error(None)}')
-  return torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+    raise RuntimeError(f'{what}: workspace query failed ({nbytes}): {N.last_error(None)}')
+  if nbytes:
+    ws = x.new_empty(nbytes, dtype=torch.uint8)
+    args.workspace, args.workspace_bytes = ws.data_ptr(), nbytes
+  _call(what, fn, x, args)
 
 
 # ---- dense ------------------------------------------------------------------------------------------------------------------------------------
@@ -64,9 +76,9 @@ def _check_dense(what, x, kernel, bias, residual, activation):
   if kernel.dim() != 2 or kernel.shape[0] != x.shape[-1] or kernel.shape[0] < 1 or kernel.shape[1] < 1:
     raise ValueError(f'{what}: kernel {tuple(kernel.shape)} does not fit x {tuple(x.shape)}: [in, out] with in = x.shape[-1] >= 1 and out >= 1')
   n = kernel.shape[1]
-  if bias is not None and tuple(bias.shape) != (n,):
+  if bias is not None and bias.shape != (n,):
     raise ValueError(f'{what}: bias {tuple(bias.shape)} for {n} outputs')
-  if residual is not None and tuple(residual.shape) != (*x.shape[:-1], n):
+  if residual is not None and residual.shape != (*x.shape[:-1], n):
     raise ValueError(f'{what}: residual {tuple(residual.shape)}, the output is {(*x.shape[:-1], n)}')
 
 
@@ -79,11 +91,11 @@ def _dense_forward(x, kernel, bias, residual, activation, keep):
   r, ldr = _rows(residual, n, one_row=True) if residual is not None else (None, 0)
   if bias is not None:
     bias = bias.contiguous()
-  m, dt, act = x2.shape[0], N.dtype_code(x.dtype), N.ACTIVATIONS[activation]
-  y = torch.empty((*x.shape[:-1], n), dtype=x.dtype, device=x.device)
+  m, dt, act = x.numel() // k, N.dtype_code(x.dtype), N.ACTIVATIONS[activation]
+  y = x.new_empty((*x.shape[:-1], n))
   save = None
   if keep and act:
-    save = torch.empty((m, (n + 7) // 8), dtype=torch.uint8, device=x.device) if activation == 'relu' else torch.empty((m, n), dtype=x.dtype, device=x.device)
+    save = x.new_empty((m, (n + 7) // 8), dtype=torch.uint8) if activation == 'relu' else x.new_empty((m, n))
   _call('nerfds_dense_forward', lib.nerfds_dense_forward, x, N.DenseForwardArgs(dt, act, m, k, n, x2.data_ptr(), ldx, w.data_ptr(), ldk, _ptr(bias), _ptr(r), ldr,
                                                                               y.data_ptr(), n, _ptr(save)))
   return y, save
@@ -98,23 +110,26 @@ def dense_backward(dy: torch.Tensor, x: torch.Tensor, kernel: torch.Tensor, save
   k, n = kernel.shape
   if tuple(dy.shape) != (*x.shape[:-1], n):
     raise ValueError(f'dense_backward: dy {tuple(dy.shape)}, the output is {(*x.shape[:-1], n)}')
-  x2, ldx = _rows(x, k)
-  m = x2.shape[0]
+  m = x.numel() // k
   if activation != 'none':
     want = (torch.uint8, (m, (n + 7) // 8)) if activation == 'relu' else (x.dtype, (m, n))
     if saved is None or saved.dtype != want[0] or tuple(saved.shape) != want[1] or saved.device != x.device or not saved.is_contiguous():
       raise ValueError(f'dense_backward: {activation} needs what dense_forward saved: a contiguous {want[0]} tensor of shape {want[1]} on {x.device}')
+  return _dense_backward(dy, x, kernel, saved if activation != 'none' else None, activation, need_dx, need_dkernel, need_dbias)
+
+
+def _dense_backward(dy, x, kernel, saved, activation, need_dx, need_dkernel, need_dbias):
   lib = N.load()
+  k, n = kernel.shape
+  x2, ldx = _rows(x, k)
   w, ldk = _rows(kernel, n)
   g, ldg = _rows(dy, n)
-  dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_dx else None
-  dkernel = torch.empty((k, n), dtype=x.dtype, device=x.device) if need_dkernel else None
-  dbias = torch.empty(n, dtype=x.dtype, device=x.device) if need_dbias else None
-  args = N.DenseBackwardArgs(N.dtype_code(x.dtype), N.ACTIVATIONS[activation], m, k, n, x2.data_ptr(), ldx, w.data_ptr(), ldk, g.data_ptr(), ldg,
-                             _ptr(saved) if activation != 'none' else None, _ptr(dx), k, _ptr(dkernel), _ptr(dbias), None, 0)
-  ws = _workspace(lib.nerfds_dense_backward_workspace(x.device.index, C.byref(args)), x)
-  args.workspace, args.workspace_bytes = _ptr(ws), ws.numel() if ws is not None else 0
-  _call('nerfds_dense_backward', lib.nerfds_dense_backward, x, args)
+  dx = x.new_empty(x.shape) if need_dx else None
+  dkernel = x.new_empty((k, n)) if need_dkernel else None
+  dbias = x.new_empty(n) if need_dbias else None
+  _call_with_workspace('nerfds_dense_backward', lib.nerfds_dense_backward_workspace, lib.nerfds_dense_backward, x,
+                       N.DenseBackwardArgs(N.dtype_code(x.dtype), N.ACTIVATIONS[activation], x.numel() // k, k, n, x2.data_ptr(), ldx, w.data_ptr(), ldk, g.data_ptr(), ldg,
+                                           _ptr(saved), _ptr(dx), k, _ptr(dkernel), _ptr(dbias), None, 0))
   return dx, dkernel, dbias
 
 
@@ -142,7 +157,7 @@ class _Dense(torch.autograd.Function):
     need = ctx.needs_input_grad
     dx = dkernel = dbias = None
     if any(need[:3]):
-      dx, dkernel, dbias = dense_backward(dy, x, kernel, saved, ctx.activation, need_dx=need[0], need_dkernel=need[1], need_dbias=need[2])
+      dx, dkernel, dbias = _dense_backward(dy, x, kernel, saved, ctx.activation, need[0], need[1], need[2])
     return dx, dkernel, dbias, dy if need[3] else None, None
 
 
@@ -162,7 +177,7 @@ def _check_norm(what, x, scale, bias, epsilon):
   if d < 1:
     raise ValueError(f'{what}: x {tuple(x.shape)} has no elements along its last axis')
   for name, t in (('scale', scale), ('bias', bias)):
-    if t is not None and tuple(t.shape) != (d,):
+    if t is not None and t.shape != (d,):
       raise ValueError(f'{what}: {name} {tuple(t.shape)} for rows of {d}')
   if not 0.0 <= epsilon < float('inf'):
     raise ValueError(f'{what}: epsilon must be finite and >= 0, got {epsilon}')
@@ -172,10 +187,11 @@ def _norm_forward(x, scale, bias, epsilon, keep):
   lib = N.load()
   d = x.shape[-1]
   x2, ldx = _rows(x, d)
-  m = x2.shape[0]
-  scale, bias = (t.contiguous() if t is not None else None for t in (scale, bias))
-  y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-  stats = torch.empty((m, 2), dtype=torch.float32, device=x.device) if keep else None
+  m = x.numel() // d
+  scale = scale.contiguous() if scale is not None else None
+  bias = bias.contiguous() if bias is not None else None
+  y = x.new_empty(x.shape)
+  stats = x.new_empty((m, 2), dtype=torch.float32) if keep else None
   _call('nerfds_layer_norm_forward', lib.nerfds_layer_norm_forward, x, N.LayerNormForwardArgs(N.dtype_code(x.dtype), d, m, epsilon, x2.data_ptr(), ldx, _ptr(scale), _ptr(bias),
                                                                                         y.data_ptr(), d, _ptr(stats)))
   return y, stats
@@ -188,21 +204,24 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, scale: Optional[torch
   _check_operands('layer_norm_backward', x, dy=dy)
   if dy.shape != x.shape:
     raise ValueError(f'layer_norm_backward: dy {tuple(dy.shape)} for x {tuple(x.shape)}')
-  d = x.shape[-1]
-  x2, ldx = _rows(x, d)
-  m = x2.shape[0]
+  m = x.numel() // x.shape[-1]
   if stats is None or tuple(stats.shape) != (m, 2) or stats.dtype != torch.float32 or stats.device != x.device or not stats.is_contiguous():
     raise ValueError(f'layer_norm_backward: stats must be the contiguous float32 [{m}, 2] tensor of layer_norm_forward')
+  return _norm_backward(dy, x, scale, stats, need_dx, need_dscale, need_dbias)
+
+
+def _norm_backward(dy, x, scale, stats, need_dx, need_dscale, need_dbias):
   lib = N.load()
+  d = x.shape[-1]
+  x2, ldx = _rows(x, d)
   g, ldg = _rows(dy, d)
   scale = scale.contiguous() if scale is not None else None
-  dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_dx else None
-  dscale = torch.empty(d, dtype=x.dtype, device=x.device) if need_dscale else None
-  dbias = torch.empty(d, dtype=x.dtype, device=x.device) if need_dbias else None
-  args = N.LayerNormBackwardArgs(N.dtype_code(x.dtype), d, m, x2.data_ptr(), ldx, _ptr(scale), g.data_ptr(), ldg, stats.data_ptr(), _ptr(dx), d, _ptr(dscale), _ptr(dbias), None, 0)
-  ws = _workspace(lib.nerfds_layer_norm_backward_workspace(x.device.index, C.byref(args)), x)
-  args.workspace, args.workspace_bytes = _ptr(ws), ws.numel() if ws is not None else 0
-  _call('nerfds_layer_norm_backward', lib.nerfds_layer_norm_backward, x, args)
+  dx = x.new_empty(x.shape) if need_dx else None
+  dscale = x.new_empty(d) if need_dscale else None
+  dbias = x.new_empty(d) if need_dbias else None
+  _call_with_workspace('nerfds_layer_norm_backward', lib.nerfds_layer_norm_backward_workspace, lib.nerfds_layer_norm_backward, x,
+                       N.LayerNormBackwardArgs(N.dtype_code(x.dtype), d, x.numel() // d, x2.data_ptr(), ldx, _ptr(scale), g.data_ptr(), ldg, stats.data_ptr(), _ptr(dx), d,
+                                               _ptr(dscale), _ptr(dbias), None, 0))
   return dx, dscale, dbias
 
 
@@ -226,7 +245,7 @@ class _LayerNorm(torch.autograd.Function):
   def backward(ctx, dy):
     x, scale, stats = ctx.saved_tensors
     need = ctx.needs_input_grad
-    return (*layer_norm_backward(dy, x, scale, stats, need_dx=need[0], need_dscale=need[1], need_dbias=need[2]), None)
+    return (*_norm_backward(dy, x, scale, stats, need[0], need[1], need[2]), None)
 
 
 def layer_norm(x: torch.Tensor, scale: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, epsilon: float = 1e-6) -> torch.Tensor:

@@ -9,6 +9,7 @@ from typing import Sequence, Union
 import torch
 
 from . import _native as N
+from .layers import _raw_stream
 
 
 def orthogonalize(updates: Union[torch.Tensor, Sequence[torch.Tensor]], steps: int = 5) -> Union[torch.Tensor, list]:
@@ -32,7 +33,7 @@ def orthogonalize(updates: Union[torch.Tensor, Sequence[torch.Tensor]], steps: i
   dt = N.dtype_code(first.dtype)
   lib = N.load()
   with torch.no_grad():
-    out = [torch.empty(u.shape, dtype=u.dtype, device=u.device) for u in mats]
+    out = [u.new_empty(u.shape) for u in mats]
     keep, entries = [], []
     for u, o in zip(mats, out):
       rows, cols = u.shape
@@ -48,8 +49,8 @@ def orthogonalize(updates: Union[torch.Tensor, Sequence[torch.Tensor]], steps: i
       nbytes = lib.nerfds_orthogonalize_workspace(arr, len(entries))
       if nbytes < 0:
         raise ValueError(f'orthogonalize: {N.last_error(None)}')
-      ws = torch.empty(nbytes, dtype=torch.uint8, device=first.device)
-      rc = lib.nerfds_orthogonalize(first.device.index, dt, arr, len(entries), int(steps), ws.data_ptr(), nbytes, torch.cuda.current_stream(first.device).cuda_stream)
+      ws = first.new_empty(nbytes, dtype=torch.uint8)
+      rc = lib.nerfds_orthogonalize(first.device.index, dt, arr, len(entries), int(steps), ws.data_ptr(), nbytes, _raw_stream(first.device.index))
       if rc != 0:
         raise RuntimeError(f'nerfds_orthogonalize failed ({rc}): {N.last_error(None)}')
   return out[0] if single else out

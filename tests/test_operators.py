@@ -87,12 +87,12 @@ def dense64(x, w, b, r, act, dy=None):
 
 def close(got, want, what=''):
   v, e = want
-  got = got.detach().cpu().double().reshape(v.shape)
+  got = got.detach().to(v.device).double().reshape(v.shape)
   bad = (got - v).abs() > e
   assert torch.isfinite(got).all() and not bad.any(), (what, int(bad.sum()), float(((got - v).abs() / e.clamp_min(1e-300)).max()))
 
 
-SHAPES = [(1, 1, 1), (1, 256, 256), (3, 7, 5), (2, 64, 3), (17, 130, 9), (130, 33, 131), (257, 560, 128), (64, 64, 64), (129, 128, 300), (1025, 45, 64)]
+SHAPES = [(1, 1, 1), (1, 256, 256), (3, 7, 5), (2, 64, 3), (5, 513, 40), (8, 1030, 77), (9, 520, 96), (17, 130, 9), (130, 33, 131), (257, 560, 128), (64, 64, 64), (129, 128, 300), (1025, 45, 64)]
 
 
 @pytest.mark.gpu
@@ -121,19 +121,30 @@ def test_dense_and_its_gradients(i, t):
       assert torch.equal(leaves[3].grad.cpu(), dy)
 
 
+# many rows past a small kernel (aligned and not), large tiles (aligned: with and without relu bits, ragged at every end), small tiles (odd sizes), few rows with splits
+MANY = [(20011, 172, 131, 'relu'), (16400, 308, 256, 'relu'), (17003, 560, 128, 'silu'), (16385, 64, 64, 'none'), (16390, 33, 70, 'softplus'), (16384, 256, 256, 'gelu'),
+        (4099, 520, 1031, 'gelu'), (4100, 520, 1056, 'relu'), (2057, 1048, 1032, 'sigmoid'), (4200, 264, 520, 'none'), (300, 1500, 70, 'none'), (2100, 1000, 96, 'relu')]
+
+
 @pytest.mark.gpu
-@pytest.mark.parametrize('t', [F32, BF16], ids=['f32', 'bf16'])
-def test_dense_at_sizes_with_many_tiles_and_splits(t):
-  for m, k, n, act in ((20011, 172, 131, 'relu'), (4099, 520, 1031, 'gelu'), (300, 1500, 70, 'none')):
-    grid = 0.25 if act == 'relu' else None
-    x, w, dy = make(m, k, t=t, seed=6, grid=grid), make(k, n, t=t, seed=7, scale=1.0 if grid else k ** -0.5, grid=grid), make(m, n, t=t, seed=8)
-    b = make(n, t=t, seed=9, grid=grid)
-    want = dense64(x, w, b, None, act, dy)
-    y, saved = layers.dense_forward(*dev(x, w, b), activation=act)
-    close(y, want['y'])
-    got = layers.dense_backward(*dev(dy, x, w), saved, act)
-    for name, g in zip(('dx', 'dkernel', 'db'), got):
-      close(g, want[name], (m, name))
+@pytest.mark.parametrize('t', [F32, F16, BF16], ids=['f32', 'f16', 'bf16'])
+@pytest.mark.parametrize('i', range(len(MANY)), ids=['%dx%dx%d-%s' % s for s in MANY])
+def test_dense_at_sizes_with_many_tiles_and_splits(i, t):
+  m, k, n, act = MANY[i]
+  grid = 0.25 if act == 'relu' else None
+  x, w, dy = make(m, k, t=t, seed=6, grid=grid), make(k, n, t=t, seed=7, scale=1.0 if grid else k ** -0.5, grid=grid), make(m, n, t=t, seed=8)
+  b = make(n, t=t, seed=9, grid=grid) if i % 4 else None
+  r = make(m, n, t=t, seed=10) if i % 2 else None
+  x, w, dy, b, r = dev(x, w, dy, b, r)      # (64-bit products of this size are the GPU's work; elementwise bounds as everywhere)
+  want = dense64(x, w, b, r, act, dy)
+  y, saved = layers.dense_forward(x, w, b, act, r)
+  close(y, want['y'])
+  for name, g in zip(('dx', 'dkernel', 'db'), layers.dense_backward(dy, x, w, saved, act)):
+    close(g, want[name], name)
+  if m % 3 == 0:      # the same through a view of padded rows
+    wide = torch.zeros((m, k + 8), dtype=t, device='cuda')
+    wide[:, :k] = x
+    assert torch.equal(layers.dense_forward(wide[:, :k], w, b, act, r)[0], y)
 
 
 @pytest.mark.gpu
