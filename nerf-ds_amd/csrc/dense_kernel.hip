@@ -74,7 +74,7 @@ template <typename T> OPS_DEV void gran_mask(Gran<T>& g, unsigned bits) {
 }
 
 // One operand's tile: 128 lines of BK contraction steps.
-//   contiguous: LDS row = line (BK elements), granule g of row r at g ^ sw(r): the 8 rows a quarter wave reads together fall on 8 different bank groups
+//   contiguous: LDS row = line (BK elements), granule g of row r at g ^ sw(r): the 16 rows that are read together fall on all 16 granules' banks
 //   strided:    LDS row = contraction step (128 elements), granule g of row r at g ^ ((r & 3) << 2), likewise for the 4 x 16 blocks of the transposed read
 template <typename T, bool CONT> struct Tile {
   static constexpr int BK = Shape<T>::BK, P = Shape<T>::P, PLANE = 128 * BK * 2, BYTES = P * PLANE;
@@ -84,7 +84,7 @@ template <typename T, bool CONT> struct Tile {
     if constexpr (CONT) { row = idx / (BK / 8); g = idx % (BK / 8); } else { row = idx / 16; g = idx % 16; }
   }
   static OPS_DEV int offset(int row, int g) {
-    if constexpr (CONT) return row * (BK * 2) + ((g ^ (BK == 64 ? row & 7 : (row >> 1) & 3)) << 4);
+    if constexpr (CONT) return row * (BK * 2) + ((g ^ (BK == 64 ? row >> 1 & 7 : row >> 2 & 3)) << 4);
     else return row * 256 + ((g ^ ((row & 3) << 2)) << 4);
   }
   // lines from `line`, contraction [c, c1)
@@ -138,19 +138,20 @@ template <typename T, bool CONT> struct Tile {
   }
 };
 
-// Activations.  For 16-bit results exp and 1 / x are the hardware's instructions (1 ulp of float32, 2^-12 of what the result keeps), log1p a series where e is
-// small, and erfc(x) = t (a1 + t (a2 + ...)) exp(-x^2), t = 1 / (1 + p x), Abramowitz & Stegun 7.1.26 (absolute error 1.5e-7): the library's erfcf is 100
-// instructions, 85 us of 33 million outputs.  float32 results take the library's functions.
+// Activations on the hardware's exp2, log2 and reciprocal (1 ulp each).  For float32 results exp's argument carries the rounding of x log2(e) along, and
+// log(1 + e) is e log(u) / (u - 1) with u = 1 + e rounded, which cancels the rounding of u: 2 - 3 ulp, where the library's expf and log1pf are 60
+// instructions (33 of 103 us for 65536 x 256 outputs).  16-bit results need neither.  erfc(x) = t (a1 + t (a2 + ...)) exp(-x^2), t = 1 / (1 + p x), is Abramowitz &
+// Stegun 7.1.26 (absolute error 1.5e-7), for 16-bit results; the library's erfcf is 100 instructions, 85 us of 33 million outputs.
 template <typename T> OPS_DEV float exp_(float x) {
-  if constexpr (sizeof(T) == 4) return expf(x); else return __builtin_amdgcn_exp2f(x * 1.44269504f);
+  const float t = x * 1.44269504f, e = __builtin_amdgcn_exp2f(t);
+  if constexpr (sizeof(T) == 2) return e;
+  const float r = fmaf(x, 1.92596299e-8f, fmaf(x, 1.44269504f, -t));      // what t lost, in units of log2: log2(e) = 1.44269504 + 1.926e-8
+  return fabsf(t) < 126.f ? fmaf(e * 0.69314718f, r, e) : e;
 }
-template <typename T> OPS_DEV float sigmoid_(float z) {
-  if constexpr (sizeof(T) == 4) return 1.f / (1.f + expf(-z)); else return __builtin_amdgcn_rcpf(1.f + exp_<T>(-z));
-}
+template <typename T> OPS_DEV float sigmoid_(float z) { return __builtin_amdgcn_rcpf(1.f + exp_<T>(-z)); }
 template <typename T> OPS_DEV float log1p_exp_(float z) {      // log(1 + exp(z)), z <= 0
-  const float e = exp_<T>(z);
-  if constexpr (sizeof(T) == 4) return log1pf(e);
-  else return e < 0.01f ? e * (1.f - e * (0.5f - e * 0.33333333f)) : 0.69314718f * __builtin_amdgcn_logf(1.f + e);      // (v_log_f32: base 2)
+  const float e = exp_<T>(z), u = 1.f + e, d = u - 1.f, l = 0.69314718f * __builtin_amdgcn_logf(u);      // (v_log_f32: base 2)
+  return d == 0.f ? e : l * e * __builtin_amdgcn_rcpf(d);
 }
 template <typename T> OPS_DEV float cdf_(float z) {            // of the normal distribution
   if constexpr (sizeof(T) == 4) return 0.5f * erfcf(-0.70710678f * z);      // (erfc: 1 + erf cancels for negative z)
@@ -161,7 +162,7 @@ template <typename T> OPS_DEV float cdf_(float z) {            // of the normal 
   }
 }
 template <typename T, int ACT> OPS_DEV float act_value(float z) {
-  if constexpr (ACT == ACT_RELU) return z > 0.f || z != z ? z : 0.f;
+  if constexpr (ACT == ACT_RELU) return z < 0.f ? 0.f : z;      // (NaN stays)
   if constexpr (ACT == ACT_SIGMOID) return sigmoid_<T>(z);
   if constexpr (ACT == ACT_SOFTPLUS) return fmaxf(z, 0.f) + log1p_exp_<T>(-fabsf(z));
   if constexpr (ACT == ACT_SILU) return z * sigmoid_<T>(z);
@@ -194,15 +195,20 @@ template <typename T> OPS_DEV void act_slopes(float (&v)[8], int act) {
   }
 }
 
+// bit j: v[j] > 0 (one compare and one add with carry each)
+OPS_DEV unsigned relu_bits(const float (&v)[8]) {
+  unsigned bits = 0;
+#pragma unroll
+  for (int j = 7; j >= 0; --j) bits = bits + bits + (v[j] > 0.f ? 1u : 0u);
+  return bits;
+}
+
 // The end of the forward for 8 elements of row m, columns n ..: what the backward needs, activation, residual, the one rounding
 template <typename T> OPS_DEV void finish(float (&v)[8], long long m, long long n, long long valid, int act, void* save, long long lds, const void* residual, long long ldr, void* y,
                                           long long ldy) {
   if (save != nullptr) {
     if (act == ACT_RELU) {
-      unsigned bits = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) bits |= (v[j] > 0.f ? 1u : 0u) << j;
-      static_cast<unsigned char*>(save)[m * lds + (n >> 3)] = (unsigned char)bits;
+      static_cast<unsigned char*>(save)[m * lds + (n >> 3)] = (unsigned char)relu_bits(v);
     } else if (act != ACT_NONE) gran_store<T>(static_cast<T*>(save) + m * lds + n, gran_pack<T>(v), valid);
   }
   act_values<T>(v, act);

@@ -16,16 +16,17 @@ OPS_DEV f32x4 mma_16(const u32x4& a, const u32x4& b, const f32x4& c, bf16_t) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-// The kernel in LDS: a row is one output line's contraction (padded to 64 steps), granules swizzled within 128 bytes for the rows that are read together.
+// The kernel in LDS: a row is one output line's contraction (padded to 64 steps).
 struct Resident {
   static __host__ __device__ int row_bytes(int c) { return (c + 63) / 64 * 128; }
   static __host__ __device__ int bytes(int n, int c) { return (n + 31) / 32 * 32 * row_bytes(c); }
-  static OPS_DEV int place(int row, int g) { return g ^ ((row & 3) | (row >> 1 & 4)); }
+  // (16 lanes read one granule of the lines 0-3, 8-11, 16-19, 24-27 of a pair together: onto the 16 granules that the banks span, in rows of 256 bytes and of 128)
+  static OPS_DEV int place(int row_bytes, int row, int g) { return g ^ (row_bytes & 128 ? (row >> 1 & 1) | (row >> 2 & 6) : (row & 3) | (row >> 1 & 12)); }
   // A pair of 16-line tiles covers 32 output lines; line i of tile `half` is output 32 pair + 8 (i >> 2) + 4 half + (i & 3), so that a lane of the accumulators
   // holds 8 consecutive outputs.  Lane l: line l & 15, contraction steps 32 ks + 8 (l >> 4) ..
   static OPS_DEV u32x4 frag(const char* lds, int row_bytes, int pair, int half, int ks) {
     const int lane = threadIdx.x & 63, i = lane & 15, row = 32 * pair + 8 * (i >> 2) + 4 * half + (i & 3);
-    return *reinterpret_cast<const u32x4*>(lds + row * row_bytes + (place(row, 4 * ks + (lane >> 4)) << 4));
+    return *reinterpret_cast<const u32x4*>(lds + row * row_bytes + (place(row_bytes, row, 4 * ks + (lane >> 4)) << 4));
   }
 };
 
@@ -40,7 +41,7 @@ template <typename T, bool BC, int NP, int OUT, bool MASK, int ACT> __global__ _
     for (int e = threadIdx.x; e < lines * grans; e += 512) {
       const int row = e / grans, g = e - row * grans;
       const Gran<T> w = gran_load<T>(static_cast<const T*>(G.b) + row * G.ldb + 8 * g, row < N ? C - 8 * g : 0);
-      *reinterpret_cast<u32x4*>(g_lds + row * row_bytes + (Resident::place(row, g) << 4)) = w.v;
+      *reinterpret_cast<u32x4*>(g_lds + row * row_bytes + (Resident::place(row_bytes, row, g) << 4)) = w.v;
     }
   } else {
     // stored with the contraction down the rows: blocks of 8 x 8 elements are transposed in registers, once
@@ -56,11 +57,12 @@ template <typename T, bool BC, int NP, int OUT, bool MASK, int ACT> __global__ _
         u32x4 out;
 #pragma unroll
         for (int i = 0; i < 4; ++i) out[i] = __builtin_amdgcn_perm(in[2 * i + 1][j >> 1], in[2 * i][j >> 1], j & 1 ? 0x07060302u : 0x05040100u);
-        *reinterpret_cast<u32x4*>(g_lds + (n + j) * row_bytes + (Resident::place(n + j, c / 8) << 4)) = out;
+        *reinterpret_cast<u32x4*>(g_lds + (n + j) * row_bytes + (Resident::place(row_bytes, n + j, c / 8) << 4)) = out;
       }
     }
   }
   __syncthreads();
+  const bool whole = N == 32 * NP;      // (bounds are checked once per 16 rows, not per granule, where nothing is ragged)
   const long long blocks = (G.M + 15) / 16, stride = (long long)gridDim.x * 8;
   long long block = (long long)blockIdx.x * 8 + wave;
   const int chunks = (C1 + 32 * KS - 1) / (32 * KS);
@@ -71,11 +73,16 @@ template <typename T, bool BC, int NP, int OUT, bool MASK, int ACT> __global__ _
     const long long m = 16 * b + (lane & 15);
     const bool in = m < G.M;
     const T* p = static_cast<const T*>(G.a) + m * G.lda + 8 * q;
+    if (16 * b + 16 <= G.M && 32 * KS * (ch + 1) <= C) {
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      const int c = 32 * (KS * ch + ks);
-      x.v[ks] = u32x4{0, 0, 0, 0};
-      if (c < C) x.v[ks] = gran_load<T>(p + c, in ? C - c - 8 * q : 0).v;
+      for (int ks = 0; ks < KS; ++ks) x.v[ks] = *reinterpret_cast<const u32x4_any*>(p + 32 * (KS * ch + ks));
+    } else {
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const int c = 32 * (KS * ch + ks);
+        x.v[ks] = u32x4{0, 0, 0, 0};
+        if (c < C) x.v[ks] = gran_load<T>(p + c, in ? C - c - 8 * q : 0).v;
+      }
     }
     if constexpr (MASK) {      // one byte per granule: 32 bytes a chunk
       const unsigned char* s = G.mask + m * G.ldm + 32 * ch;
@@ -103,12 +110,18 @@ template <typename T, bool BC, int NP, int OUT, bool MASK, int ACT> __global__ _
       for (int p = 0; p < NP; ++p) acc[p][0] = acc[p][1] = f32x4{0.f, 0.f, 0.f, 0.f};
       if constexpr (OUT == OUT_FORWARD) {
         if (G.residual != nullptr) {
+          const T* p0 = static_cast<const T*>(G.residual) + m * G.ldr + 8 * q;
+          if (whole && 16 * block + 16 <= G.M) {
 #pragma unroll
-          for (int p = 0; p < NP; ++p) r[p] = gran_load<T>(static_cast<const T*>(G.residual) + m * G.ldr + 32 * p + 8 * q, m < G.M ? N - 32 * p - 8 * q : 0);
+            for (int p = 0; p < NP; ++p) r[p].v = *reinterpret_cast<const u32x4_any*>(p0 + 32 * p);
+          } else {
+#pragma unroll
+            for (int p = 0; p < NP; ++p) r[p] = gran_load<T>(p0 + 32 * p, m < G.M ? N - 32 * p - 8 * q : 0);
+          }
         }
       }
     }
-    const bool wrap = ch + 1 == chunks;
+    const bool wrap = ch + 1 == chunks, all = whole && 16 * block + 16 <= G.M;
     if (!wrap || block + stride < blocks) fetch(next, wrap ? block + stride : block, wrap ? 0 : ch + 1);
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
@@ -143,15 +156,15 @@ template <typename T, bool BC, int NP, int OUT, bool MASK, int ACT> __global__ _
       if constexpr (OUT == OUT_FORWARD) {
         if (G.save != nullptr) {
           if constexpr (ACT == ACT_RELU) {
-            unsigned bits = 0;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) bits |= (v[e] > 0.f && n + e < N ? 1u : 0u) << e;
             // the 4 bytes of the pair's 32 outputs, put together over the four lanes of a row; lane q keeps the dwords q and q + 4
-            unsigned w = bits << (8 * q);
+            unsigned w = relu_bits(v) << (8 * q);      // (columns past N: the kernel's padding is 0, and so are they)
             w |= __shfl_xor(w, 16, 64);
             w |= __shfl_xor(w, 32, 64);
             if ((p & 3) == q) relu[p >> 2] = w;
-          } else if constexpr (ACT != ACT_NONE) gran_store<T>(static_cast<T*>(G.save) + m * G.lds + n, gran_pack<T>(v), valid);
+          } else if constexpr (ACT != ACT_NONE) {
+            if (all) *reinterpret_cast<u32x4_any*>(static_cast<T*>(G.save) + m * G.lds + n) = gran_pack<T>(v).v;
+            else gran_store<T>(static_cast<T*>(G.save) + m * G.lds + n, gran_pack<T>(v), valid);
+          }
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = act_value<T, ACT>(v[e]);
@@ -160,7 +173,8 @@ template <typename T, bool BC, int NP, int OUT, bool MASK, int ACT> __global__ _
           for (int e = 0; e < 8; ++e) v[e] += gran_get<T>(r[p], e);
         }
       }
-      gran_store<T>(static_cast<T*>(G.y) + m * G.ldy + n, gran_pack<T>(v), valid);
+      if (all) *reinterpret_cast<u32x4_any*>(static_cast<T*>(G.y) + m * G.ldy + n) = gran_pack<T>(v).v;
+      else gran_store<T>(static_cast<T*>(G.y) + m * G.ldy + n, gran_pack<T>(v), valid);
     }
     if constexpr (OUT == OUT_FORWARD && ACT == ACT_RELU) {
       if (G.save != nullptr && in) {

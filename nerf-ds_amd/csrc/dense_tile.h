@@ -28,9 +28,8 @@ template <int LINES_, bool CONT_, bool PERM> struct Stage {
   static constexpr int ROWG = CONT ? BK / 8 : LINES / 8;      // granules of an LDS row
   static_assert(INSTR % 8 == 0, "whole instructions for 8 waves");
   static OPS_DEV int swz(int row) {
-    if constexpr (!CONT) return (row & 3) << 2;
-    else if constexpr (PERM) return ((row >> 1) & 1) | ((row >> 2) & 2);      // (the rows a quarter wave reads are 0-3 and 8-11, 4-7 and 12-15)
-    else return (row >> 1) & 3;
+    // (16 lanes read together: 16 lines at one step, 4 to the 256 bytes that the banks span; or 4 steps of 4 granules)
+    return CONT ? row >> 2 & 3 : (row & 3) << 2;
   }
   // this lane's granule of DMA instruction u of its wave
   static OPS_DEV void place(int u, int& row, int& g) {
@@ -283,10 +282,7 @@ template <typename T, typename GR, bool AC, bool BC, int OUT, int MASK, int ACT>
               for (int e = 0; e < 8; ++e) v[e] += bias[j][d][e];
               if (G.save != nullptr) {
                 if constexpr (ACT == ACT_RELU) {
-                  unsigned bits = 0;
-#pragma unroll
-                  for (int e = 0; e < 8; ++e) bits |= (v[e] > 0.f ? 1u : 0u) << e;
-                  relu[j & 1] |= bits << (16 * d);
+                  relu[j & 1] |= relu_bits(v) << (16 * d);
                 } else if (ACT != ACT_NONE && in) gran_store<T>(static_cast<T*>(G.save) + m * G.lds + n, gran_pack<T>(v), 8);
               }
 #pragma unroll

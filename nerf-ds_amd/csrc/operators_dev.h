@@ -61,12 +61,18 @@ template <typename T> OPS_DEV float gran_get(const Gran<T>& g, int i) {
   if constexpr (sizeof(T) == 4) return g.v[i >> 2][i & 3];
   else return to_f32<T>(__builtin_bit_cast(T, (uint16_t)(g.v[i >> 1] >> (16 * (i & 1)))));
 }
+template <typename T> struct Pair;      // two elements, for the conversions that take two
+template <> struct Pair<f16_t> { typedef __attribute__((ext_vector_type(2))) _Float16 type; };
+template <> struct Pair<bf16_t> { typedef __attribute__((ext_vector_type(2))) __bf16 type; };
 template <typename T> OPS_DEV Gran<T> gran_pack(const float (&f)[8]) {
   Gran<T> g = gran_zero<T>();
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    if constexpr (sizeof(T) == 4) g.v[i >> 2][i & 3] = f[i];
-    else g.v[i >> 1] |= (unsigned)__builtin_bit_cast(uint16_t, from_f32<T>(f[i])) << (16 * (i & 1));
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 4) { g.v[i >> 1][2 * (i & 1)] = f[2 * i]; g.v[i >> 1][2 * (i & 1) + 1] = f[2 * i + 1]; }
+    else {
+      typedef __attribute__((ext_vector_type(2))) float f32x2;
+      g.v[i] = __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2{f[2 * i], f[2 * i + 1]}), typename Pair<T>::type));
+    }
   }
   return g;
 }

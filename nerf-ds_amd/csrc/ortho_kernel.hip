@@ -182,7 +182,7 @@ OPS_DEV f32x16 mma16(const u32x4& a, const u32x4& b, const f32x16& c) {
 // LDS tiles of f16: a row is one line's BK contraction steps.  Granules of 16 bytes are swizzled so that the rows one read touches together fall on different
 // banks.  (Every product has the contraction along the rows of both operands - X X^T, A A^T = A A, B (X^T)^T - because X is kept beside its
 // transpose: a transposed read of LDS makes the compiler wait for every DMA in flight.)
-template <int ROWB> OPS_DEV int swizzle(int row) { return ROWB == 128 ? row & 7 : (row >> 1) & 3; }
+template <int ROWB> OPS_DEV int swizzle(int row) { return ROWB == 128 ? row >> 1 & 7 : row >> 2 & 3; }
 template <int ROWB> OPS_DEV u32x4 tile_frag(const char* lds, int t, int ks) {
   const int lane = threadIdx.x & 63, row = 32 * t + (lane & 31), g = 2 * ks + (lane >> 5);
   return *reinterpret_cast<const u32x4*>(lds + row * ROWB + ((g ^ swizzle<ROWB>(row)) << 4));
@@ -210,7 +210,7 @@ template <int STEP, typename T, int TS> __global__ __launch_bounds__(WAVES8) voi
   constexpr int BK = R::BK, W = TS / 64;      // 32 x 32 tiles per wave and side
   constexpr bool SYM = STEP == GRAM || STEP == POLY;
   constexpr int ROWB = BK * 2;
-  const Found at = find(B, SYM ? (int)blockIdx.x : (int)xcd_order(blockIdx.x, gridDim.x));
+  const Found at = find(B, blockIdx.x);
   const Mat& M = B.m[at.i];
   const Layout L(M.rows, M.cols, TS);
   int t = at.local, ti, tj;
@@ -219,7 +219,8 @@ template <int STEP, typename T, int TS> __global__ __launch_bounds__(WAVES8) voi
     ti = 0;
     while (t >= tn - ti) { t -= tn - ti; ++ti; }
     tj = ti + t;
-  } else {      // bands of 8 tile rows, down the band first: the 32 tiles in flight on an XCD are then 8 x 4 and share operands both ways
+  } else {      // bands of 8 tile rows, down the band first, a stretch of them per XCD: the 32 tiles in flight there are 8 x 4 and share operands both ways
+    t = (int)xcd_order(t, (L.np / TS) * (L.mp / TS));
     const int tn = L.np / TS, tm = L.mp / TS, band = t / (8 * tm), rows = min(8, tn - 8 * band), r = t - band * 8 * tm;
     ti = 8 * band + r % rows;
     tj = r / rows;
@@ -288,11 +289,18 @@ template <int STEP, typename T, int TS> __global__ __launch_bounds__(WAVES8) voi
   const _Float16* add = STEP == POLY ? A : X;
   const int ld = SYM ? L.np : L.mp;
   const long long plane = SYM ? aplane : xplane;
+  // a wave takes 16 rows x 4 granules: 64 bytes of a row in memory, and 32 of a column in the transposed planes (2 waves' worth of banks)
+  auto mine = [&](int u, int& r, int& c) __attribute__((always_inline)) {
+    const int b = (threadIdx.x >> 6) + 8 * u;
+    r = 16 * (b % (TS / 16)) + (lane >> 2);
+    c = 8 * (4 * (b / (TS / 16)) + (lane & 3));
+  };
   Gran<f16_t> old[EACH][2];
 #pragma unroll
   for (int u = 0; u < EACH; ++u) {
-    const int e = threadIdx.x + WAVES8 * u;
-    const _Float16* at = add + (long long)(i0 + e / GR) * ld + j0 + e % GR * 8;
+    int r, c;
+    mine(u, r, c);
+    const _Float16* at = add + (long long)(i0 + r) * ld + j0 + c;
     if constexpr (STEP != GRAM) { old[u][0].v = *reinterpret_cast<const u32x4*>(at); old[u][1].v = *reinterpret_cast<const u32x4*>(at + plane); }
   }
   // 1. float32, the even and the odd steps' sums
@@ -319,7 +327,9 @@ template <int STEP, typename T, int TS> __global__ __launch_bounds__(WAVES8) voi
   _Float16* out = STEP == GRAM ? A : STEP == POLY ? P : reinterpret_cast<_Float16*>(ws + L.x(cur ^ 1));
 #pragma unroll
   for (int u = 0; u < EACH; ++u) {
-    const int e = threadIdx.x + WAVES8 * u, r = e / GR, c = e % GR * 8, i = i0 + r, j = j0 + c;
+    int r, c;
+    mine(u, r, c);
+    const int i = i0 + r, j = j0 + c;
     if (SYM && W == 2 && ti == tj && r >= 64 && c < 64) continue;      // (the mirror image of the block above the diagonal: written in 3.)
     const long long at = (long long)i * ld + j;
     float v[8];
@@ -390,9 +400,11 @@ template <typename T> __global__ __launch_bounds__(WAVES8) void k_whole(const Ba
   char* A = g_lds + 2 * xplane;
   char* P = A + 2 * 8192;
   f32x4* even = reinterpret_cast<f32x4*>(P + 2 * 8192);      // [4 waves][4 quads][64 lanes]: the even steps' sums of a symmetric product
-  // X is read along its rows (GRAM) and across them (UPDATE, transposed): granule g of row r sits at g ^ (r & 7) within its 128-byte block, which serves both
-  auto xat = [&](int r, int g) __attribute__((always_inline)) { return r * rowx + ((g ^ (r & 7)) << 4); };
-  auto aat = [&](int r, int g) __attribute__((always_inline)) { return r * 128 + ((g ^ (r & 7)) << 4); };
+  // X is read along its rows (16 lines, one granule) and across them (4 rows, 4 granules, transposed): the swizzle sends both to the 16 granules that the banks
+  // span, in rows of 128 bytes (modulo 256) and of 256
+  auto turn8 = [](int r) __attribute__((always_inline)) { return (r << 1 & 4) | (r >> 2 & 3); };
+  auto xat = [&](int r, int g) __attribute__((always_inline)) { return r * rowx + ((g ^ (rowx & 128 ? turn8(r) : (r << 2 & 12) | (r >> 2 & 3))) << 4); };
+  auto aat = [&](int r, int g) __attribute__((always_inline)) { return r * 128 + ((g ^ turn8(r)) << 4); };
 
   double* red = reinterpret_cast<double*>(g_lds);
   double* parts = red + THREADS;
@@ -562,6 +574,7 @@ template <typename T, int TS> void products(hipStream_t st, Batch& B, int count,
 
 template <typename T> void run(hipStream_t st, const OrthoMat* mats, int count, int steps, char* ws) {
   const Ways ways(mats, count);
+  // (the longest contractions first in each batch: what is left at a launch's end is then short)
   for (const Way way : {WHOLE, TILES_64, TILES_128}) {
     for (int at = 0; at < count;) {
       Batch B{};
@@ -578,6 +591,7 @@ template <typename T> void run(hipStream_t st, const OrthoMat* mats, int count, 
       }
       ws += off;
       if (n == 0) break;
+      if (way != WHOLE) std::stable_sort(B.m, B.m + n, [](const Mat& a, const Mat& b) { return std::min(a.rows, a.cols) > std::min(b.rows, b.cols); });
       if (way == WHOLE) {
         nerfds::allow_dynamic_lds(reinterpret_cast<const void*>(&k_whole<T>), WHOLE_LDS);
         hipLaunchKernelGGL((k_whole<T>), dim3((unsigned)n), dim3(WAVES8), WHOLE_LDS, st, B, steps);

@@ -151,14 +151,21 @@ class _Dense(torch.autograd.Function):
     return y
 
   @staticmethod
-  @once_differentiable
   def backward(ctx, dy):
+    return _dense_gradients_once(ctx, dy) if torch.is_grad_enabled() else _Dense.gradients(ctx, dy)
+
+  @staticmethod
+  def gradients(ctx, dy):
     x, kernel, saved = ctx.saved_tensors
     need = ctx.needs_input_grad
     dx = dkernel = dbias = None
     if any(need[:3]):
       dx, dkernel, dbias = _dense_backward(dy, x, kernel, saved, ctx.activation, need[0], need[1], need[2])
     return dx, dkernel, dbias, dy if need[3] else None, None
+
+
+# with create_graph=True the gradients come out marked as not differentiable again (the mark costs more than the launch, so it is left out otherwise)
+_dense_gradients_once = once_differentiable(_Dense.gradients)
 
 
 def dense(x: torch.Tensor, kernel: torch.Tensor, bias: Optional[torch.Tensor] = None, activation: str = 'none', residual: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -241,11 +248,17 @@ class _LayerNorm(torch.autograd.Function):
     return y
 
   @staticmethod
-  @once_differentiable
   def backward(ctx, dy):
+    return _norm_gradients_once(ctx, dy) if torch.is_grad_enabled() else _LayerNorm.gradients(ctx, dy)
+
+  @staticmethod
+  def gradients(ctx, dy):
     x, scale, stats = ctx.saved_tensors
     need = ctx.needs_input_grad
     return (*_norm_backward(dy, x, scale, stats, need[0], need[1], need[2]), None)
+
+
+_norm_gradients_once = once_differentiable(_LayerNorm.gradients)
 
 
 def layer_norm(x: torch.Tensor, scale: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, epsilon: float = 1e-6) -> torch.Tensor:

@@ -3,7 +3,7 @@ nerfds_orthogonalize), all matrices of a call together whatever their shapes.  `
 field's own hidden kernels; this is the same operator for a caller's matrices.  No CPU path."""
 from __future__ import annotations
 
-import ctypes as C
+import struct
 from typing import Sequence, Union
 
 import torch
@@ -23,34 +23,40 @@ def orthogonalize(updates: Union[torch.Tensor, Sequence[torch.Tensor]], steps: i
   if not mats:
     return []
   first = mats[0]
-  for u in mats:
-    if not isinstance(u, torch.Tensor) or u.dim() != 2:
-      raise ValueError('orthogonalize: every update must be a 2-d tensor')
-    if not u.is_cuda:
-      raise RuntimeError('orthogonalize runs on the GPU: the updates must be CUDA tensors (there is no CPU path)')
-    if u.dtype != first.dtype or u.device != first.device:
-      raise ValueError(f'orthogonalize: one element type and device per call, got {u.dtype} on {u.device} next to {first.dtype} on {first.device}')
-  dt = N.dtype_code(first.dtype)
-  lib = N.load()
+  if not isinstance(first, torch.Tensor):
+    raise ValueError('orthogonalize: every update must be a 2-d tensor')
+  dtype, index = first.dtype, first.get_device()
+  out, keep, fields = [], [], []
   with torch.no_grad():
-    out = [u.new_empty(u.shape) for u in mats]
-    keep, entries = [], []
-    for u, o in zip(mats, out):
+    for u in mats:
+      if not isinstance(u, torch.Tensor) or u.dim() != 2:
+        raise ValueError('orthogonalize: every update must be a 2-d tensor')
+      if not u.is_cuda:
+        raise RuntimeError('orthogonalize runs on the GPU: the updates must be CUDA tensors (there is no CPU path)')
+      if u.dtype != dtype or u.get_device() != index:
+        raise ValueError(f'orthogonalize: one element type and device per call, got {u.dtype} on {u.device} next to {dtype} on {first.device}')
       rows, cols = u.shape
+      o = u.new_empty((rows, cols))
+      out.append(o)
       if rows == 0 or cols == 0:
         continue
-      ld = u.stride(0) if rows > 1 else cols
-      if (cols > 1 and u.stride(1) != 1) or ld < cols:
+      ld, one = u.stride()
+      if rows == 1:
+        ld = cols
+      if (cols > 1 and one != 1) or ld < cols:
         u, ld = u.contiguous(), cols
         keep.append(u)
-      entries.append((u.data_ptr(), ld, o.data_ptr(), cols, rows, cols))
-    if entries:
-      arr = (N.Matrix * len(entries))(*entries)
-      nbytes = lib.nerfds_orthogonalize_workspace(arr, len(entries))
+      fields += (u.data_ptr(), ld, o.data_ptr(), cols, rows, cols)
+    code = N.dtype_code(dtype)
+    count = len(fields) // 6
+    if count:
+      lib = N.load()
+      mats_c = (N.Matrix * count).from_buffer_copy(struct.pack('PqPqii' * count, *fields))
+      nbytes = lib.nerfds_orthogonalize_workspace(mats_c, count)
       if nbytes < 0:
         raise ValueError(f'orthogonalize: {N.last_error(None)}')
-      ws = first.new_empty(nbytes, dtype=torch.uint8)
-      rc = lib.nerfds_orthogonalize(first.device.index, dt, arr, len(entries), int(steps), ws.data_ptr(), nbytes, _raw_stream(first.device.index))
+      ws = first.new_empty(max(nbytes, 1), dtype=torch.uint8)
+      rc = lib.nerfds_orthogonalize(index, code, mats_c, count, int(steps), ws.data_ptr(), nbytes, _raw_stream(index))
       if rc != 0:
         raise RuntimeError(f'nerfds_orthogonalize failed ({rc}): {N.last_error(None)}')
   return out[0] if single else out

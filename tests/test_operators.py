@@ -516,10 +516,11 @@ def test_python_refusals_on_the_gpu():
   for f, text in cases:
     with pytest.raises(ValueError, match=text):
       f()
-  y = layers.dense(x.requires_grad_(True), w)
-  (g,) = torch.autograd.grad(y, x, torch.ones_like(y), create_graph=True)
-  with pytest.raises(RuntimeError):      # first order only
-    g.sum().backward()
+  x.requires_grad_(True)
+  for y in (layers.dense(x, w), layers.layer_norm(x, w[:, 0].contiguous())):      # first order only, and said so
+    (g,) = torch.autograd.grad(y, x, torch.ones_like(y), create_graph=True)
+    with pytest.raises(RuntimeError):
+      g.sum().backward()
 
 
 def test_c_refusals():
@@ -568,12 +569,12 @@ def test_c_refusals():
   assert fwd(m=0, x=None) == 0 and nfwd(m=0, y=None) == 0
 
   def ortho(dtype=0, count=1, steps=5, ws=p, nbytes=1 << 20, **kw):
-    mat = N.Matrix(p, 4, p, 4, 4, 4)
+    mat = N.Matrix(p, 100, p, 100, 100, 100)      # (large enough to need a workspace)
     for k, v in kw.items():
       setattr(mat, k, v)
     return lib.nerfds_orthogonalize(0, dtype, C.byref(mat), count, steps, ws, nbytes, None)
   for kw in (dict(dtype=9), dict(count=-1), dict(steps=0), dict(steps=17), dict(ws=None), dict(ws=p + 8), dict(nbytes=16), dict(rows=0), dict(cols=-1), dict(rows=40000), dict(u=None),
-             dict(ldu=3), dict(ldo=3), dict(o=p + 1)):
+             dict(ldu=99), dict(ldo=99), dict(o=p + 1)):
     assert ortho(**kw) == EINVAL, kw
   assert ortho(count=0) == 0 and lib.nerfds_orthogonalize(0, 0, None, 1, 5, p, 1 << 20, None) == EINVAL
   assert lib.nerfds_dense_save_bytes(1, 1, 5, 9) == 10 and lib.nerfds_dense_save_bytes(0, 5, 5, 9) == 180 and lib.nerfds_dense_save_bytes(2, 0, 5, 9) == 0
