@@ -241,7 +241,7 @@ int nerfds_abi_version(void);
 /* sizeof the public structs as THIS library was compiled, for a binding to check its own declarations against (host only):
  * which = 0 nerfds_model_cfg, 1 nerfds_weights, 2 nerfds_camera, 3 nerfds_rays, 4 nerfds_extra, 5 nerfds_rand, 6 nerfds_out,
  * 7 nerfds_train_objective, 8 nerfds_train_numerics, 9 / 10 nerfds_dense_forward_args / _backward_args, 11 / 12 nerfds_layer_norm_forward_args /
- * _backward_args, 13 nerfds_matrix; anything else: -1. */
+ * _backward_args, 13 nerfds_matrix, 14 nerfds_optimizer; anything else: -1. */
 int64_t nerfds_struct_size(int which);
 /* The arithmetic (NERFDS_PREC_BF16 / BF16X3 / F32 / F16) each network runs in under a NERFDS_PREC_* value of this build:
  * plan_out = {MaskMLP, SE3 warp field, hyper sheet, NerfMLP trunk (+ alpha head), rgb branch}.  Uniform for every value
@@ -364,6 +364,24 @@ int nerfds_trainer_upload(nerfds_trainer* t, int which, const float* host);
 /* target_norm = normalize(R normalize(-d sigma_raw / d x)) per sample (models.py:1069-1077, 1273-1277, 1328; 'warped' supervision) of the
  * last step run with NERFDS_TRAIN_SIGMA_GRAD: HOST [num_rays][S][3], S = Nc (level 0) or Nc + Nf (level 1). */
 int nerfds_trainer_target_norm(nerfds_trainer* t, int level, int64_t num_rays, float* host);
+/* The update that nerfds_trainer_step / nerfds_trainer_apply make.  NERFDS_OPTIMIZER_ADAM (the default; the other fields are not read): flax.optim.Adam on
+ * every leaf.  NERFDS_OPTIMIZER_MUON: the kernels between hidden layers (.../hidden_i/kernel, bottleneck/kernel) take an orthogonalised momentum step -
+ *   m <- momentum m + g;  u = g + momentum m (nesterov) or m;  O = orthogonalised u (nerfds_orthogonalize, `steps` steps)
+ *   W <- W (1 - lr weight_decay) - lr 0.2 sqrt(max(rows, cols)) O
+ * - and all other leaves Adam's, under one learning rate (the factor gives O the RMS of an Adam update).  m is kept where Adam's first moment would be
+ * (nerfds_trainer_download which = 2); the second moment of these leaves stays 0.  A non-finite gradient skips the whole update as under Adam.  No
+ * reference counterpart (train.py:297-301 knows Adam only).  Choosing an optimizer resets its state and the step count. */
+#define NERFDS_OPTIMIZER_ADAM 0
+#define NERFDS_OPTIMIZER_MUON 1
+typedef struct nerfds_optimizer {
+  int32_t kind;              /* NERFDS_OPTIMIZER_* */
+  float momentum;            /* [0, 1); 0.95 is usual */
+  int32_t nesterov;          /* 0 / 1 */
+  int32_t steps;             /* 1 .. 16; 5 is usual */
+  float weight_decay;        /* >= 0, of the orthogonalised leaves */
+} nerfds_optimizer;
+int nerfds_trainer_set_optimizer(nerfds_trainer* t, const nerfds_optimizer* optimizer);
+int nerfds_trainer_leaf_optimizer(const nerfds_trainer* t, int index);   /* NERFDS_OPTIMIZER_* of a leaf under the optimizer chosen; negative: no such leaf */
 int nerfds_trainer_reset_optimizer(nerfds_trainer* t);   /* zero the Adam moments and the step count */
 int nerfds_trainer_set_step(nerfds_trainer* t, int64_t step);   /* the optimizer's step count (resuming from a checkpoint: OptimizerState.step) */
 /* The optimizer's step count = the number of updates actually APPLIED (it lives on the device and does not advance on an update skipped for a

@@ -298,6 +298,7 @@ int64_t nerfds_struct_size(int which) {
     case 11: return sizeof(nerfds_layer_norm_forward_args);
     case 12: return sizeof(nerfds_layer_norm_backward_args);
     case 13: return sizeof(nerfds_matrix);
+    case 14: return sizeof(nerfds_optimizer);
     default: return -1;
   }
 }

@@ -21,6 +21,7 @@
 #include "nerfds.h"
 #include "train_kernels.h"
 #include "train_gemm.h"
+#include "operators.h"
 #include "graphs.h"
 #include "kargs.h"
 #include "pack.h"
@@ -75,6 +76,14 @@ struct nerfds_trainer {
   float *theta = nullptr, *grad = nullptr, *m1 = nullptr, *m2 = nullptr;
   // the optimizer's step count + the bias corrections of the update being applied, on the DEVICE (train_kernels.hip k_adam_prepare): 8 + 2 x 4 bytes
   unsigned char* adam_dev = nullptr;
+  // nerfds_trainer_set_optimizer: the hidden kernels' update orthogonalised (ortho_kernel.hip) instead of Adam's.  u: their updates, one after the other;
+  // blocks: the leaves in pieces for the element-wise passes; allocated when the optimizer is first chosen, kept until the end
+  nerfds_optimizer opt{NERFDS_OPTIMIZER_ADAM, 0.f, 0, 0, 0.f};
+  std::vector<nerfds_ops::OrthoMat> ortho;
+  float* ortho_u = nullptr;
+  char* ortho_work = nullptr;
+  nerfds_ops::UpdateBlock* blocks_dev = nullptr;
+  int num_blocks = 0;
   long long* adam_step() const { return reinterpret_cast<long long*>(adam_dev); }
   float* adam_corr() const { return reinterpret_cast<float*>(adam_dev + 8); }
   // a caller-defined loss (nerfds_trainer_forward / nerfds_render_rays_bwd): per level (0 coarse, 1 fine) the cotangents that replace the squared error's
@@ -231,6 +240,9 @@ struct nerfds_trainer {
     for (int i = 0; i < 5; ++i) if (pstream16[i]) (void)hipFree(pstream16[i]);
     for (int i = 0; i < 2; ++i) if (tstream16[i]) (void)hipFree(tstream16[i]);
     if (adam_dev) (void)hipFree(adam_dev);
+    if (ortho_u) (void)hipFree(ortho_u);
+    if (ortho_work) (void)hipFree(ortho_work);
+    if (blocks_dev) (void)hipFree(blocks_dev);
     if (wpack) (void)hipFree(wpack);
     if (grad_rep) (void)hipFree(grad_rep);
     for (int i = 0; i < SIDE; ++i) { if (side[i]) (void)hipStreamDestroy(side[i]); if (join_ev[i]) (void)hipEventDestroy(join_ev[i]); }
@@ -2163,10 +2175,71 @@ int nerfds_trainer_reset_optimizer(nerfds_trainer* t) {
   return NERFDS_OK;
 }
 
+// The leaves whose update is orthogonalised under NERFDS_OPTIMIZER_MUON: kernels between hidden layers.  First layers' inputs are encodings and the heads'
+// outputs a handful of numbers, but both are matrices of the same kind here; embeddings, heads (logit) and biases stay with Adam.
+static bool orthogonalized_leaf(const Leaf& l) {
+  const bool kernel = l.name.size() > 7 && l.name.compare(l.name.size() - 7, 7, "/kernel") == 0;
+  return kernel && (l.name.find("/hidden_") != std::string::npos || l.name.find("/bottleneck/") != std::string::npos);
+}
+
+int nerfds_trainer_leaf_optimizer(const nerfds_trainer* t, int index) {
+  if (!t || index < 0 || index >= (int)t->leaves.size()) return NERFDS_EINVAL;
+  return t->opt.kind == NERFDS_OPTIMIZER_MUON && orthogonalized_leaf(t->leaves[index]) ? NERFDS_OPTIMIZER_MUON : NERFDS_OPTIMIZER_ADAM;
+}
+
+static int set_optimizer(nerfds_trainer* t, const nerfds_optimizer* o) {
+  if (!o || (o->kind != NERFDS_OPTIMIZER_ADAM && o->kind != NERFDS_OPTIMIZER_MUON)) return t->fail(NERFDS_EINVAL, "nerfds_trainer_set_optimizer: unknown optimizer");
+  if (o->kind == NERFDS_OPTIMIZER_MUON && (!(o->momentum >= 0.f && o->momentum < 1.f) || o->steps < 1 || o->steps > 16 || !(o->weight_decay >= 0.f) || std::isinf(o->weight_decay)))
+    return t->fail(NERFDS_EINVAL, "nerfds_trainer_set_optimizer: 0 <= momentum < 1, 1 <= steps <= 16, 0 <= weight_decay (got %g, %d, %g)", o->momentum, o->steps, o->weight_decay);
+  if (hipSetDevice(t->device) != hipSuccess) return t->fail(NERFDS_EDEVICE, "hipSetDevice failed");
+  if (o->kind == NERFDS_OPTIMIZER_MUON && !t->ortho_u) {
+    std::vector<nerfds_ops::UpdateBlock> blocks;
+    std::vector<int64_t> at;
+    int64_t total = 0;
+    for (const Leaf& l : t->leaves) {
+      const bool orth = orthogonalized_leaf(l);
+      const int64_t count = (int64_t)l.rows * l.cols;
+      for (int64_t i = 0; i < count; i += 1024)
+        blocks.push_back({l.off + i, orth ? total + i : -1, (int)std::min<int64_t>(1024, count - i), orth ? 0.2f * std::sqrt((float)std::max(l.rows, l.cols)) : 0.f});
+      if (orth) { at.push_back(total); total += (count + 63) & ~int64_t(63); }
+    }
+    std::vector<nerfds_ops::OrthoMat> mats;
+    for (const Leaf& l : t->leaves)
+      if (orthogonalized_leaf(l)) mats.push_back({nullptr, l.cols, nullptr, l.cols, l.rows, l.cols});
+    float* u = nullptr;
+    char* work = nullptr;
+    nerfds_ops::UpdateBlock* dev = nullptr;
+    const size_t ub = (size_t)total * sizeof(float), wb = nerfds_ops::ortho_ws(mats.data(), (int)mats.size()), bb = blocks.size() * sizeof(blocks[0]);
+    if (hipMalloc(&u, ub) != hipSuccess || hipMalloc(&work, wb + 256) != hipSuccess || hipMalloc(&dev, bb) != hipSuccess || hipMemset(u, 0, ub) != hipSuccess ||
+        hipMemcpy(dev, blocks.data(), bb, hipMemcpyHostToDevice) != hipSuccess) {
+      for (void* p : {(void*)u, (void*)work, (void*)dev}) if (p) (void)hipFree(p);
+      (void)hipGetLastError();
+      return t->fail(NERFDS_ENOMEM, "hipMalloc failed (orthogonalised update: %zu bytes)", ub + wb + bb);
+    }
+    for (size_t i = 0; i < mats.size(); ++i) mats[i].u = mats[i].o = u + at[i];
+    t->ortho_u = u; t->ortho_work = work; t->blocks_dev = dev; t->num_blocks = (int)blocks.size(); t->ortho = std::move(mats);
+  }
+  t->opt = *o;
+  return nerfds_trainer_reset_optimizer(t);
+}
+int nerfds_trainer_set_optimizer(nerfds_trainer* t, const nerfds_optimizer* o) {
+  if (!t) return NERFDS_EINVAL;
+  try {
+    return set_optimizer(t, o);
+  } catch (const std::exception&) { return NERFDS_ENOMEM; }      // (the lists of leaves)
+}
+
 static void adam_update(nerfds_trainer* t, float learning_rate, hipStream_t st) {
   unsigned* flag = reinterpret_cast<unsigned*>(t->terms_dev + 8);
   (void)hipMemsetAsync(flag, 0, sizeof(unsigned), st);
   // the step count advances on the device, and only if the update is applied (a skipped update leaves parameters, moments AND the count alone)
+  if (t->opt.kind == NERFDS_OPTIMIZER_MUON) {
+    adam_begin(st, t->grad, t->P, 0.9f, 0.999f, t->adam_step(), t->adam_corr(), flag);
+    nerfds_ops::muon_momentum(st, t->blocks_dev, t->num_blocks, t->grad, t->m1, t->ortho_u, t->opt.momentum, t->opt.nesterov, flag);
+    nerfds_ops::orthogonalize(st, nerfds_ops::F32, t->ortho.data(), (int)t->ortho.size(), t->opt.steps, t->ortho_work);
+    nerfds_ops::muon_update(st, t->blocks_dev, t->num_blocks, t->grad, t->ortho_u, t->theta, t->m1, t->m2, learning_rate, t->opt.weight_decay, t->adam_corr(), flag);
+    return;
+  }
   adam(st, t->theta, t->grad, t->m1, t->m2, t->P, learning_rate, 0.9f, 0.999f, 1e-8f, t->adam_step(), t->adam_corr(), flag);
 }
 

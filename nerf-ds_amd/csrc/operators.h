@@ -62,4 +62,12 @@ struct OrthoMat { const void* u; long long ldu; void* o; long long ldo; int rows
 size_t ortho_ws(const OrthoMat* mats, int count);
 void orthogonalize(hipStream_t st, int dtype, const OrthoMat* mats, int count, int steps, void* ws);
 
+
+// ---- the trainer's update with orthogonalised kernels (muon_kernel.hip) --------------------------------------------------------------------
+// up to 1024 elements of one leaf, from `offset` of the flat vectors; u >= 0: an orthogonalised leaf, its update starts at u of the update buffer
+struct UpdateBlock { long long offset, u; int count; float scale; };
+void muon_momentum(hipStream_t st, const UpdateBlock* blocks, int count, const float* g, float* m, float* u, float beta, int nesterov, const unsigned* skip);
+void muon_update(hipStream_t st, const UpdateBlock* blocks, int count, const float* g, const float* o, float* p, float* m1, float* m2, float lr, float wd, const float* corr,
+                 const unsigned* skip);
+
 }  // namespace nerfds_ops

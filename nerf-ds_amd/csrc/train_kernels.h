@@ -91,6 +91,8 @@ void se3_jvp(hipStream_t, long long M, const float* wv, const float* x, const fl
 void trunk_in_jvp(hipStream_t, const Dims&, long long M, const float* xw, const float* wamb, const float* t_xw, const float* t_wamb, const Windows&, float* t_tin, int rp = 3);
 void target_norm(hipStream_t, long long M, const float* t_alpha, const float* wv, float* out);
 void clip_gradients(hipStream_t, float* g, long long n, float max_val, float max_norm, float* sumsq_scratch);
+// the first half of adam(): raises the flag if a gradient element is not finite, otherwise advances the step count and its bias corrections
+void adam_begin(hipStream_t, const float* g, long long n, float b1, float b2, long long* step_dev, float* corr_dev, unsigned* nonfinite_flag);
 void adam(hipStream_t, float* p, const float* g, float* m1, float* m2, long long n, float lr, float b1, float b2, float eps, long long* step_dev,
           float* corr_dev, unsigned* nonfinite_flag);      // flag != 0 after the gradient check: nothing is updated
 // fused forward: weight streams / biases / folded rgb layer from the current parameters (see train_kernels.hip)

@@ -1473,10 +1473,13 @@ void clip_gradients(hipStream_t st, float* g, long long n, float max_val, float 
   LAUNCH(k_clip_val_sumsq, n, st, g, n, max_val, sumsq_scratch);
   if (max_norm > 0.f) LAUNCH(k_clip_norm, n, st, g, n, max_norm, 1e-7f, sumsq_scratch);
 }
-void adam(hipStream_t st, float* p, const float* g, float* m1, float* m2, long long n, float lr, float b1, float b2, float eps, long long* step_dev,
-          float* corr_dev, unsigned* nonfinite_flag) {
+void adam_begin(hipStream_t st, const float* g, long long n, float b1, float b2, long long* step_dev, float* corr_dev, unsigned* nonfinite_flag) {
   LAUNCH(k_nonfinite, n, st, g, n, nonfinite_flag);
   hipLaunchKernelGGL(k_adam_prepare, dim3(1), dim3(1), 0, st, nonfinite_flag, step_dev, corr_dev, (double)b1, (double)b2);
+}
+void adam(hipStream_t st, float* p, const float* g, float* m1, float* m2, long long n, float lr, float b1, float b2, float eps, long long* step_dev,
+          float* corr_dev, unsigned* nonfinite_flag) {
+  adam_begin(st, g, n, b1, b2, step_dev, corr_dev, nonfinite_flag);
   LAUNCH(k_adam, n, st, p, g, m1, m2, n, lr, b1, b2, eps, corr_dev, nonfinite_flag);
 }
 

@@ -171,6 +171,12 @@ class Matrix(C.Structure):
   _fields_ = [('u', C.c_void_p), ('ldu', C.c_int64), ('o', C.c_void_p), ('ldo', C.c_int64), ('rows', C.c_int32), ('cols', C.c_int32)]
 
 
+class Optimizer(C.Structure):
+  _fields_ = [('kind', C.c_int32), ('momentum', C.c_float), ('nesterov', C.c_int32), ('steps', C.c_int32), ('weight_decay', C.c_float)]
+
+
+OPTIMIZERS = {'adam': 0, 'muon': 1}
+
 # every symbol include/nerfds.h declares
 SYMBOLS = ('nerfds_abi_version', 'nerfds_struct_size', 'nerfds_precision_plan', 'nerfds_precision_plan_level', 'nerfds_ctx_create', 'nerfds_ctx_load_weights', 'nerfds_render_rays',
            'nerfds_encode_embed', 'nerfds_ctx_destroy', 'nerfds_last_error', 'nerfds_kernel_time_ms', 'nerfds_pack_stream_bytes', 'nerfds_pack_stream_bytes_level',
@@ -181,7 +187,8 @@ SYMBOLS = ('nerfds_abi_version', 'nerfds_struct_size', 'nerfds_precision_plan', 
            'nerfds_trainer_last_error', 'nerfds_trainer_debug_read', 'nerfds_trainer_nonfinite', 'nerfds_trainer_set_step', 'nerfds_trainer_get_step', 'nerfds_trainer_set_loss_scale_adjust', 'nerfds_trainer_set_numerics', 'nerfds_trainer_get_numerics', 'nerfds_trainer_overflow_sources', 'nerfds_trainer_forward', 'nerfds_render_rays_bwd',
            'nerfds_debug_lds_attr_first_use',
            'nerfds_dense_save_bytes', 'nerfds_dense_backward_workspace', 'nerfds_dense_forward', 'nerfds_dense_backward', 'nerfds_layer_norm_forward',
-           'nerfds_layer_norm_backward_workspace', 'nerfds_layer_norm_backward', 'nerfds_orthogonalize_workspace', 'nerfds_orthogonalize')
+           'nerfds_layer_norm_backward_workspace', 'nerfds_layer_norm_backward', 'nerfds_orthogonalize_workspace', 'nerfds_orthogonalize',
+           'nerfds_trainer_set_optimizer', 'nerfds_trainer_leaf_optimizer')
 
 _lib = None
 
@@ -241,7 +248,7 @@ def load():
   for f in (lib.nerfds_dense_save_bytes, lib.nerfds_dense_backward_workspace, lib.nerfds_layer_norm_backward_workspace, lib.nerfds_orthogonalize_workspace):
     f.restype = C.c_int64
   structs = {i: st for i, st in enumerate((ModelCfg, Weights, CameraStruct, Rays, Extra, Rand, Out))}
-  structs.update({9: DenseForwardArgs, 10: DenseBackwardArgs, 11: LayerNormForwardArgs, 12: LayerNormBackwardArgs, 13: Matrix})
+  structs.update({9: DenseForwardArgs, 10: DenseBackwardArgs, 11: LayerNormForwardArgs, 12: LayerNormBackwardArgs, 13: Matrix, 14: Optimizer})
   for which, st in structs.items():      # the ctypes mirrors against the library's own sizeof
     if lib.nerfds_struct_size(which) != C.sizeof(st):
       raise RuntimeError(f'{st.__name__}: ctypes declares {C.sizeof(st)} bytes, libnerfds_hip.so has {lib.nerfds_struct_size(which)} (include/nerfds.h changed?)')

@@ -73,6 +73,8 @@ def _bind(lib):
   lib.nerfds_trainer_grads.argtypes = [C.c_void_p]
   lib.nerfds_trainer_grads.restype = C.c_void_p
   lib.nerfds_trainer_reset_optimizer.argtypes = [C.c_void_p]
+  lib.nerfds_trainer_set_optimizer.argtypes = [C.c_void_p, C.POINTER(N.Optimizer)]
+  lib.nerfds_trainer_leaf_optimizer.argtypes = [C.c_void_p, C.c_int]
   lib.nerfds_trainer_set_step.argtypes = [C.c_void_p, C.c_int64]
   lib.nerfds_trainer_get_step.argtypes = [C.c_void_p, C.POINTER(C.c_int64)]
   lib.nerfds_trainer_set_loss_scale_adjust.argtypes = [C.c_void_p, C.c_int32]
@@ -99,10 +101,11 @@ class Trainer:
   """Owns the flat fp32 parameter / gradient / Adam vectors on one MI355X."""
 
   def __init__(self, cfg: NerfModelConfig, params: Optional[Dict[str, Any]] = None, max_rays: int = 4096,
-               device: Optional[torch.device] = None, warp_embeds=None):
+               device: Optional[torch.device] = None, warp_embeds=None, optimizer: str = 'adam', optimizer_options: Optional[Dict[str, Any]] = None):
     """``warp_embeds``: the list of warp ids present in the dataset (model.warp_embeds = embeddings_dict['warp'], models.py:248-250): what the
     background regulariser draws its random ids from (training.py:163).  None = range(num_warp_embeds), which is the same thing when the
-    training ids are contiguous from 0 - with sparse ids it would regularise GLO rows no ray ever trains."""
+    training ids are contiguous from 0 - with sparse ids it would regularise GLO rows no ray ever trains.
+    ``optimizer``, ``optimizer_options``: as ``set_optimizer(optimizer, **optimizer_options)``."""
     cfg.validate()
     self.cfg = cfg
     self.warp_embeds = None if warp_embeds is None else torch.as_tensor(np.asarray(list(warp_embeds)).astype(np.int64)).reshape(-1)
@@ -145,6 +148,26 @@ class Trainer:
       self.leaves.append((name.value.decode(), off.value, rows.value, cols.value))
     if params is not None:
       self.set_params(params)
+    self.optimizer = 'adam'
+    if optimizer != 'adam' or optimizer_options:
+      self.set_optimizer(optimizer, **(optimizer_options or {}))
+
+  def set_optimizer(self, kind: str, momentum: float = 0.95, nesterov: bool = True, steps: int = 5, weight_decay: float = 0.0) -> None:
+    """What ``step`` / ``apply_gradients`` do with the gradient (include/nerfds.h nerfds_trainer_set_optimizer): 'adam' on every leaf, or 'muon' - an
+    orthogonalised momentum update (``optim.orthogonalize``) on the kernels between hidden layers (``orthogonalized_leaves``), Adam on the rest, one
+    learning rate for both.  Resets the optimizer's state.  ``get_opt_state`` holds the momentum in place of the first moment of those leaves."""
+    if kind not in N.OPTIMIZERS:
+      raise ValueError(f'unknown optimizer {kind!r} (one of {", ".join(N.OPTIMIZERS)})')
+    o = N.Optimizer(N.OPTIMIZERS[kind], float(momentum), int(bool(nesterov)), int(steps), float(weight_decay))
+    rc = self._lib.nerfds_trainer_set_optimizer(self._h, C.byref(o))
+    if rc != 0:
+      raise (ValueError if rc == -22 else RuntimeError)(f'nerfds_trainer_set_optimizer failed ({rc}): {(self._lib.nerfds_trainer_last_error(self._h) or b"").decode()}')
+    self.optimizer = kind
+
+  @property
+  def orthogonalized_leaves(self):
+    """Names of the leaves whose update is orthogonalised under the optimizer chosen."""
+    return [name for i, (name, *_) in enumerate(self.leaves) if self._lib.nerfds_trainer_leaf_optimizer(self._h, i) == N.OPTIMIZERS['muon']]
 
   def __del__(self):
     h = getattr(self, '_h', None)

@@ -587,3 +587,84 @@ def test_struct_sizes_of_the_operators():
   lib = N.load()
   for which, st in ((9, N.DenseForwardArgs), (10, N.DenseBackwardArgs), (11, N.LayerNormForwardArgs), (12, N.LayerNormBackwardArgs), (13, N.Matrix)):
     assert lib.nerfds_struct_size(which) == C.sizeof(st)
+
+
+# ---- the trainer's orthogonalised update -----------------------------------------------------------------------------------------------------------
+def _trainer(**kw):
+  from nerfds_amd import init_params, nerf_ds_config
+  from nerfds_amd.training import Trainer
+  cfg = nerf_ds_config(num_warp_embeds=4, num_coarse_samples=8, num_fine_samples=8)
+  return Trainer(cfg, init_params(cfg, 0, warp_head_scale=5e-2, small_head_scale=0.3, bias_scale=0.1), max_rays=64, **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('nesterov', [True, False])
+def test_trainer_with_orthogonalised_kernels(nesterov):
+  beta, wd, lr = 0.9, 0.1, 1e-2
+  muon = _trainer(optimizer='muon', optimizer_options=dict(momentum=beta, nesterov=nesterov, weight_decay=wd))
+  adam = _trainer()
+  names = muon.orthogonalized_leaves
+  assert len(names) == 40 and 'nerf_mlps_fine/bottleneck/kernel' in names and adam.orthogonalized_leaves == []
+  assert all('/hidden_' in n or 'bottleneck' in n for n in names) and not any('logit' in n or 'bias' in n or 'embed' in n for n in names)
+  leaves = {name: (off, rows, cols) for name, off, rows, cols in muon.leaves}
+  m = {n: 0.0 for n in names}
+  w = {n: muon.params_tensor()[leaves[n][0]:leaves[n][0] + leaves[n][1] * leaves[n][2]].cpu().double().reshape(leaves[n][1:]) for n in names}
+  for step in range(3):
+    g = make(muon.num_params, seed=step, scale=1e-3).cuda()
+    for tr in (muon, adam):
+      tr.grads_tensor().copy_(g)
+      torch.cuda.synchronize()
+      tr.apply_gradients(lr)
+    got, ref, first = (x.cpu() for x in (muon.params_tensor(), adam.params_tensor(), g))
+    ema = torch.as_tensor(muon._download(2))
+    rest = torch.ones(muon.num_params, dtype=torch.bool)
+    for n in names:
+      off, rows, cols = leaves[n]
+      gi = first[off:off + rows * cols].double().reshape(rows, cols)
+      m[n] = beta * m[n] + gi
+      o = ortho64((gi + beta * m[n] if nesterov else m[n]))
+      w[n] = w[n] * (1 - lr * wd) - lr * 0.2 * math.sqrt(max(rows, cols)) * o
+      err = got[off:off + rows * cols].double().reshape(rows, cols) - w[n]
+      assert float(err.norm()) < float((step + 1) * (4 * E24 * w[n].norm() + lr * 0.2 * math.sqrt(max(rows, cols)) * (ortho_bound(F32) + 8 * E24) * o.norm())), n
+      assert float((ema[off:off + rows * cols].double().reshape(rows, cols) - m[n]).abs().max()) <= 4 * E24 * float(m[n].abs().max())
+      rest[off:off + rows * cols] = False
+    # the other leaves: Adam's formula in another kernel, whose multiply-adds may be fused elsewhere: per step the moments differ by 2 roundings each, quotient,
+    # root and product by 4 more, the update (at most lr / sqrt(1 - b2) / ... = 3.2 lr in three steps) by 8 x 2^-24 of itself, the parameter by one
+    assert float((got[rest] - ref[rest]).abs().max()) <= (step + 1) * E24 * (8 * 3.2 * lr + float(ref[rest].abs().max()))
+  assert muon.optimizer_step == 3 and not muon.nonfinite()
+  before, moments = muon._download(0), muon._download(2)
+  g[5] = float('inf')
+  muon.grads_tensor().copy_(g)
+  torch.cuda.synchronize()
+  muon.apply_gradients(lr)
+  assert muon.nonfinite() and muon.optimizer_step == 3 and (muon._download(0) == before).all() and (muon._download(2) == moments).all()
+  muon.set_optimizer('adam')
+  assert muon.optimizer_step == 0 and not muon._download(2).any() and muon.orthogonalized_leaves == []
+
+
+@pytest.mark.gpu
+def test_trainer_steps_and_resumes_with_orthogonalised_kernels():
+  import numpy as np
+  rng = np.random.default_rng(0)
+  d = rng.normal(size=(64, 3))
+  d /= np.linalg.norm(d, axis=-1, keepdims=True)
+  batch = dict(origins=rng.normal(size=(64, 3)) * 0.1, directions=d, rgb=rng.random((64, 3)), metadata={'warp': rng.integers(0, 4, (64, 1))}, mask=np.zeros((64, 1)))
+  extra = dict(nerf_alpha=8., warp_alpha=4., hyper_alpha=1., hyper_sheet_alpha=6., norm_input_alpha=4.)
+  a, b = _trainer(optimizer='muon'), _trainer(optimizer='muon')
+  a.step(batch, extra, 1e-3, seed=1)
+  b.set_params(a.get_params())
+  b.set_opt_state(*a.get_opt_state(), a.optimizer_step)
+  for tr in (a, b):
+    stats = tr.step(batch, extra, 1e-3, seed=2)
+    assert math.isfinite(stats['loss/total']) and tr.optimizer_step == 2
+  # The step's gradients are sums of float32 atomics, equal up to their order: 1e-5 of a kernel's gradient at the most, which the orthogonalisation
+  # multiplies by 3.4445^5 = 485 at the most: 5e-3 of an element of O, times lr 0.2 sqrt(560) = 4.7e-3 (and again for the momentum: 5e-5)
+  pa, pb = a._download(0), b._download(0)
+  for name, off, rows, cols in a.leaves:
+    if name in a.orthogonalized_leaves:
+      assert np.abs(pa[off:off + rows * cols] - pb[off:off + rows * cols]).max() < 5e-5, name
+  for kw in (dict(momentum=1.0), dict(momentum=-0.1), dict(steps=0), dict(steps=17), dict(weight_decay=-1.0), dict(weight_decay=float('nan')), dict(momentum=float('nan'))):
+    with pytest.raises(ValueError):
+      a.set_optimizer('muon', **kw)
+  with pytest.raises(ValueError, match='unknown optimizer'):
+    a.set_optimizer('sgd')
