@@ -195,15 +195,15 @@ extern __shared__ __attribute__((aligned(16))) char g_lds[];
 // all but the newest N loads have arrived, and this wave's LDS reads too: past the barrier that follows, the stage they came from may be overwritten
 template <int N> OPS_DEV void wait_loads() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory"); }
 
-// One TS x TS tile of a product; GRAM and POLY are symmetric: tiles i <= j only, written twice.  Operand tiles arrive by LDS-DMA, RING stages of 32 KiB
-// deep, one barrier a stage.  8 waves: four of (TS / 2) x (TS / 2) take the even, four the odd contraction steps of 16, and their sums are added - two waves
+// One TS x TS tile of a product; GRAM and POLY are symmetric: tiles i <= j only, written twice.  Operand tiles arrive by LDS-DMA, 128 KiB of them under way
+// or in use (128-byte rows: a request then is a whole cache line, half as many as with rows of 64), one barrier a stage.  8 waves: four of (TS / 2) x (TS / 2) take the even, four the odd contraction steps of 16, and their sums are added - two waves
 // per SIMD, so that one's LDS reads run under the other's MFMAs, without reading any fragment more often.
 template <int TS> struct Ring {
-  static constexpr int BK = TS == 64 ? 64 : 32, PLANE = TS * BK * 2, STAGE = 4 * PLANE, COUNT = 4, IPW = STAGE / 1024 / 8;
+  static constexpr int BK = 64, PLANE = TS * BK * 2, STAGE = 4 * PLANE, COUNT = TS == 64 ? 4 : 2, IPW = STAGE / 1024 / 8, EACH = IPW / 4;      // DMA instructions per wave: of a stage, of a plane
   // afterwards: the tile in float32, and its two planes transposed (rows padded against bank conflicts)
   static constexpr int ROWF = TS + 4, ROWT = TS + 8, OUTF = TS * ROWF * 4, OUTT = TS * ROWT * 2;
   static constexpr int LDS = COUNT * STAGE > OUTF + 2 * OUTT ? COUNT * STAGE : OUTF + 2 * OUTT;
-  static_assert(STAGE == 32768 && IPW == 4, "an instruction per wave and plane");
+  static_assert(IPW == 4 * EACH, "whole instructions per wave and plane");
 };
 template <int STEP, typename T, int TS> __global__ __launch_bounds__(WAVES8) void k_product(const Batch B, int cur) {
   typedef Ring<TS> R;
@@ -237,16 +237,22 @@ template <int STEP, typename T, int TS> __global__ __launch_bounds__(WAVES8) voi
   const long long pl = STEP == GRAM ? xplane : aplane, pr = STEP == POLY ? aplane : xplane;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wi = wave >> 1 & 1, wj = wave & 1, odd = wave >> 2;
 
-  // DMA: wave w fills bytes 1024 w .. of each plane, in the order left hi, left lo, right hi, right lo
-  const int drow = (wave * 64 + lane) / (ROWB / 16), dg = (lane % (ROWB / 16)) ^ swizzle<ROWB>(drow);
-  const _Float16* src[2] = {lhs + (long long)(i0 + drow) * K + 8 * dg, rhs + (long long)(j0 + drow) * K + 8 * dg};
+  // DMA: instruction u of wave w fills bytes 1024 (w + 8 u) .. of each plane, planes in the order left hi, left lo, right hi, right lo
+  const _Float16* src[2][R::EACH];
+#pragma unroll
+  for (int u = 0; u < R::EACH; ++u) {
+    const int slot = (wave + 8 * u) * 64 + lane, row = slot / (ROWB / 16), g = (slot % (ROWB / 16)) ^ swizzle<ROWB>(row);
+    src[0][u] = lhs + (long long)(i0 + row) * K + 8 * g;
+    src[1][u] = rhs + (long long)(j0 + row) * K + 8 * g;
+  }
   const int steps = K / BK;
   auto issue = [&](int s, int slot) __attribute__((always_inline)) {
     s = s < steps ? s : steps - 1;      // (past the end: the last one again, into a slot nobody reads any more, so that the waits can count)
 #pragma unroll
     for (int u = 0; u < R::IPW; ++u) {
-      const _Float16* g = src[u >> 1] + s * BK + (u & 1 ? (u >> 1 ? pr : pl) : 0);
-      const int off = __builtin_amdgcn_readfirstlane(slot * R::STAGE + u * R::PLANE + wave * 1024);
+      const int plane = u / R::EACH, e = u % R::EACH;
+      const _Float16* g = src[plane >> 1][e] + s * BK + (plane & 1 ? (plane >> 1 ? pr : pl) : 0);
+      const int off = __builtin_amdgcn_readfirstlane(slot * R::STAGE + plane * R::PLANE + (wave + 8 * e) * 1024);
       __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g, (__attribute__((address_space(3))) void*)(g_lds + off), 16, 0, 0);
     }
   };
