@@ -348,6 +348,7 @@ __global__ __launch_bounds__(THREADS, 2) void k_gemm(const GemmArgs G) {
 
 #include "dense_tile.h"
 #include "dense_resident.h"
+#include "dense_backward.h"
 
 // The forward of a few rows (m <= 8: one frame's embedding, one token): bound by reading the kernel once, so by how many loads are in flight.  A workgroup
 // takes 32 columns - a cache line's worth of every kernel row - and all of k: thread (slice, granule) multiplies 8 rows of 8 columns at a time, and
@@ -423,19 +424,30 @@ bool weight_tiles_large(const DenseBwd& w) {
   return w.act != ACT_RELU || (w.n % 32 == 0 && reinterpret_cast<uintptr_t>(w.save) % 4 == 0);
 }
 
+// Whether both gradients come from one pass (k_both): a narrow layer in 16 bits and both wanted.  It was faster at every number of rows tried, 16 to 524288
+// (256 x 256 in bf16: 16 us instead of 10 + 11 at 16 rows, 28 instead of 9 + 26 at 4096, 213 instead of 119 + 130 at 524288).
+bool both_at_once(const DenseBwd& w) { return w.dx != nullptr && w.dkernel != nullptr && w.k <= 256 && w.n <= 256 && weight_tiles_large(w); }
+
 struct Splits { int count; long long cps; };
 // The weight gradient has few output tiles (1 for 256 x 256) and a long contraction: as many splits as fill the card - one workgroup per CU of the large tiles,
-// two of the small ones -, none shorter than 256 rows.  A fraction of a round more is no gain: splits are rounded down there.
+// two of the small ones.  A fraction of a round more is no gain: splits are rounded down there.  Few rows are cut short too, for each split is one chain of loads
+// and products: into 64 rows while all parts together stay under 8 MB, else 128 (256 x 256 in float32 at 512 rows: 11 us with 64, 15 with 128, 22 with 256; in
+// bf16 at 4096 rows, where 64 would make 16 MB: 25, 23 and 26).  k_both, which makes dx too, takes 64 (8192 rows in bf16: 37 us with 32, 32 with 64, 33 with 128).
 Splits weight_splits(const DenseBwd& w, int num_cus) {
+  const long long steps = up(w.m, 64);
+  if (both_at_once(w)) return {(int)(steps < num_cus ? steps : num_cus), 0};
   const bool large = weight_tiles_large(w);
-  const long long tiles = large ? up(w.k, 256) * up(w.n, w.n > 128 ? 256 : 128) : up(w.k, BM) * up(w.n, BN), slots = large ? num_cus : 2LL * num_cus, steps = up(w.m, 64);
+  const long long tiles = large ? up(w.k, 256) * up(w.n, w.n > 128 ? 256 : 128) : up(w.k, BM) * up(w.n, BN), slots = large ? num_cus : 2LL * num_cus;
   long long want = tiles >= slots ? 1 : slots / tiles;
-  if (want > up(steps, 4)) want = up(steps, 4);
+  const long long most = steps <= (2 << 20) / ((long long)w.k * w.n) ? steps : up(steps, 2);
+  if (want > most) want = most;
   const long long cps = up(steps, want) * 64;
   return {(int)up(w.m, cps), cps};
 }
 
-size_t weight_part_bytes(int splits, long long kn) { return splits > 1 ? aligned((size_t)splits * up(kn, 4) * 16) : 0; }      // (one split writes the result itself)
+size_t weight_part_bytes(const DenseBwd& w, int splits) {      // (one split of the weight gradient alone writes the result itself)
+  return splits > 1 || both_at_once(w) ? aligned((size_t)splits * up((long long)w.k * w.n, 4) * 16) : 0;
+}
 
 // Whether k_tile can take the product: rows of whole, aligned granules on both sides (M, N and C too where they run along rows), relu bits in whole dwords
 template <bool AC, bool BC, int MASK> bool tile_fits(const GemmArgs& G) {
@@ -506,6 +518,18 @@ template <typename T> void forward_t(hipStream_t st, const DenseFwd& f, int num_
   launch<T, true, false, OUT_FORWARD, 0>(st, G, num_cus);
 }
 
+template <typename T, int KP, int NP, bool MASK> void launch_both(hipStream_t st, const BothArgs& G, int grid) {
+  auto kern = k_both<T, KP, NP, MASK>;
+  nerfds::allow_dynamic_lds(reinterpret_cast<const void*>(kern), Both<KP, NP>::LDS);
+  hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(512), (Both<KP, NP>::LDS), st, G);
+}
+template <typename T, bool MASK> void launch_both_of(hipStream_t st, const BothArgs& G, int grid) {
+  if (G.k > 128 && G.n > 128) launch_both<T, 256, 256, MASK>(st, G, grid);
+  else if (G.k > 128) launch_both<T, 256, 128, MASK>(st, G, grid);
+  else if (G.n > 128) launch_both<T, 128, 256, MASK>(st, G, grid);
+  else launch_both<T, 128, 128, MASK>(st, G, grid);
+}
+
 template <typename T> void backward_t(hipStream_t st, const DenseBwd& w, int num_cus) {
   char* ws = static_cast<char*>(w.ws);
   const void* dz = w.dy;
@@ -518,6 +542,18 @@ template <typename T> void backward_t(hipStream_t st, const DenseBwd& w, int num
     ws += aligned((size_t)w.m * w.n * sizeof(T));
   }
   const unsigned char* bits = w.act == ACT_RELU ? static_cast<const unsigned char*>(w.save) : nullptr;
+  if constexpr (sizeof(T) == 2) {
+    if (both_at_once(w)) {
+      const int grid = weight_splits(w, num_cus).count;
+      const long long kn = (long long)w.k * w.n;
+      float* part = reinterpret_cast<float*>(ws);
+      float* col = reinterpret_cast<float*>(ws + weight_part_bytes(w, grid));
+      const BothArgs G{w.x, w.ldx, dz, lddz, w.kernel, w.ldk, bits, up(w.n, 8), w.dx, w.lddx, part, w.dbias ? col : nullptr, w.m, w.k, w.n};
+      if (bits) launch_both_of<T, true>(st, G, grid); else launch_both_of<T, false>(st, G, grid);
+      sum_splits<T>(st, SplitSum{part, up(kn, 4) * 4, kn, w.dkernel}, SplitSum{col, up(w.n, 4) * 4, w.n, w.dbias}, grid);
+      return;
+    }
+  }
   if (w.dx != nullptr) {
     GemmArgs G{};
     G.a = dz; G.lda = lddz; G.b = w.kernel; G.ldb = w.ldk; G.M = w.m; G.N = w.k; G.C = w.n;
@@ -531,7 +567,7 @@ template <typename T> void backward_t(hipStream_t st, const DenseBwd& w, int num
     G.M = w.dkernel ? w.k : 1;      // (the bias gradient alone: it rides on the first tile of the kernel's rows)
     G.mask = bits; G.ldm = up(w.n, 8); G.splits = s.count; G.cps = s.cps;
     const long long kn = (long long)w.k * w.n;
-    const size_t part_bytes = weight_part_bytes(s.count, kn);
+    const size_t part_bytes = weight_part_bytes(w, s.count);
     G.part = w.dkernel && s.count > 1 ? reinterpret_cast<float*>(ws) : nullptr;
     if (s.count == 1) { G.y = w.dkernel; G.ldy = w.n; }
     float* col = reinterpret_cast<float*>(ws + part_bytes);
@@ -549,7 +585,7 @@ size_t dense_save_bytes(int dtype, int act, long long m, int n) {
 size_t dense_bwd_ws(const DenseBwd& a, int num_cus) {
   const Splits s = weight_splits(a, num_cus);
   size_t b = a.act != ACT_NONE && a.act != ACT_RELU ? aligned((size_t)a.m * a.n * dtype_bytes(a.dtype)) : 0;
-  if (a.dkernel != nullptr || a.dbias != nullptr) b += weight_part_bytes(s.count, (long long)a.k * a.n) + aligned((size_t)s.count * up(a.n, 4) * 16);
+  if (a.dkernel != nullptr || a.dbias != nullptr) b += weight_part_bytes(a, s.count) + aligned((size_t)s.count * up(a.n, 4) * 16);
   return b;
 }
 void dense_forward(hipStream_t st, const DenseFwd& a, int num_cus) {

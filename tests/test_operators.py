@@ -147,6 +147,30 @@ def test_dense_at_sizes_with_many_tiles_and_splits(i, t):
     assert torch.equal(layers.dense_forward(wide[:, :k], w, b, act, r)[0], y)
 
 
+# both gradients in one pass: each width class, a last stage of a few rows or of one, several rounds of the ring of stages, one workgroup
+BOTH = [(32768, 256, 256, 'relu'), (150001, 256, 256, 'relu'), (140003, 160, 136, 'gelu'), (140033, 256, 96, 'relu'), (90001, 200, 64, 'none'), (90007, 64, 256, 'relu'), (33000, 128, 200, 'silu'),
+        (100001, 96, 128, 'relu'), (70000, 128, 8, 'none'),
+        (1, 256, 256, 'relu'), (63, 256, 256, 'none'), (65, 128, 160, 'relu'), (500, 8, 32, 'relu')]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('t', [F16, BF16], ids=['f16', 'bf16'])
+@pytest.mark.parametrize('i', range(len(BOTH)), ids=['%dx%dx%d-%s' % s for s in BOTH])
+def test_dense_gradients_of_narrow_layers(i, t):
+  m, k, n, act = BOTH[i]
+  grid = 0.25 if act == 'relu' else None
+  x, w, dy = dev(make(m, k, t=t, seed=6, grid=grid), make(k, n, t=t, seed=7, scale=1.0 if grid else k ** -0.5, grid=grid), make(m, n, t=t, seed=8))
+  want = dense64(x, w, None, None, act, dy)
+  _, saved = layers.dense_forward(x, w, None, act)
+  first = layers.dense_backward(dy, x, w, saved, act)
+  for name, g in zip(('dx', 'dkernel', 'db'), first):
+    close(g, want[name], name)
+  again = layers.dense_backward(dy, x, w, saved, act, need_dbias=False)
+  assert torch.equal(again[0], first[0]) and torch.equal(again[1], first[1]) and again[2] is None
+  close(layers.dense_backward(dy, x, w, saved, act, need_dkernel=False)[0], want['dx'], 'dx')      # apart, by other kernels
+  close(layers.dense_backward(dy, x, w, saved, act, need_dx=False)[1], want['dkernel'], 'dkernel')
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize('t', [F32, F16], ids=['f32', 'f16'])
 def test_dense_takes_views_expanded_residuals_and_leading_axes(t):
