@@ -395,21 +395,26 @@ template <typename T, int M> __global__ __launch_bounds__(256) void k_rows(const
   finish<T>(v, m, n, valid, A.act, A.save, A.act == ACT_RELU ? (A.n + 7) / 8 : A.n, A.residual, A.ldr, A.y, A.ldy);
 }
 
-// dz = dy act'(z), once, for the activations whose slope costs more than a bit test (the products below read dz once per tile of their other axis).
-// dz is rounded to the tensors' type: the matrix pipe takes it in no other.
-template <typename T> __global__ __launch_bounds__(256) void k_dz(const T* __restrict__ dy, long long lddy, const T* __restrict__ z, T* __restrict__ dz, long long m, int n, int act) {
+// dz = dy act'(z), once, for the activations whose slope costs more than a bit test (the products below read dz once per tile of their other axis), and for relu
+// (z: its bits) where those tiles are many.  dz is rounded to the tensors' type: the matrix pipe takes it in no other.
+template <typename T, bool RELU> __global__ __launch_bounds__(256) void k_dz(const T* __restrict__ dy, long long lddy, const void* __restrict__ z, T* __restrict__ dz, long long m, int n, int act) {
   const int gn = (n + 7) / 8;
   for (long long i = blockIdx.x * 256LL + threadIdx.x; i < m * gn; i += gridDim.x * 256LL) {
     const long long row = i / gn;
     const int c = (int)(i % gn) * 8;
-    const Gran<T> a = gran_load<T>(dy + row * lddy + c, n - c), b = gran_load<T>(z + row * n + c, n - c);
-    float v[8];
+    Gran<T> a = gran_load<T>(dy + row * lddy + c, n - c);
+    if constexpr (RELU) gran_mask<T>(a, static_cast<const unsigned char*>(z)[i]);
+    else {
+      const Gran<T> b = gran_load<T>(static_cast<const T*>(z) + row * n + c, n - c);
+      float v[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = gran_get<T>(b, j);
-    act_slopes<T>(v, act);
+      for (int j = 0; j < 8; ++j) v[j] = gran_get<T>(b, j);
+      act_slopes<T>(v, act);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] *= gran_get<T>(a, j);
-    gran_store<T>(dz + row * n + c, gran_pack<T>(v), n - c);
+      for (int j = 0; j < 8; ++j) v[j] *= gran_get<T>(a, j);
+      a = gran_pack<T>(v);
+    }
+    gran_store<T>(dz + row * n + c, a, n - c);
   }
 }
 
@@ -417,11 +422,17 @@ long long up(long long a, long long b) { return (a + b - 1) / b; }
 size_t aligned(size_t b) { return (b + 255) & ~(size_t)255; }
 
 bool whole_granules(const void* p, long long ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0; }
-// whether the weight gradient can go through k_tile: its operands' rows are whole, aligned granules, relu bits whole dwords (a smooth activation's dz is ours)
+// Whether dz is written to the workspace before the products.  Relu: where they run on large tiles, of which every column (k / 256) tests the bits of the same
+// dy again (8192 x 2048 -> 4096: 170 + 207 us for dx and dkernel, and 20 + 132 + 151 with a stored dz; at k = 512 the two ways cost the same).
+bool stores_dz(const DenseBwd& w) {
+  if (w.act == ACT_NONE || w.act == ACT_RELU) return w.act == ACT_RELU && w.dtype != F32 && w.k > (w.dx && w.dkernel ? 512 : 1024) && w.k % 8 == 0 && w.n % 8 == 0 && whole_granules(w.x, w.ldx);
+  return true;
+}
+// whether the weight gradient can go through k_tile: its operands' rows are whole, aligned granules, relu bits whole dwords (a dz in the workspace is)
 bool weight_tiles_large(const DenseBwd& w) {
   if (w.dtype == F32 || w.k % 8 || w.n % 8 || !whole_granules(w.x, w.ldx)) return false;
-  if (w.act == ACT_NONE || w.act == ACT_RELU) { if (!whole_granules(w.dy, w.lddy)) return false; }
-  return w.act != ACT_RELU || (w.n % 32 == 0 && reinterpret_cast<uintptr_t>(w.save) % 4 == 0);
+  if (stores_dz(w)) return true;
+  return whole_granules(w.dy, w.lddy) && (w.act != ACT_RELU || (w.n % 32 == 0 && reinterpret_cast<uintptr_t>(w.save) % 4 == 0));
 }
 
 // Whether both gradients come from one pass (k_both): a narrow layer in 16 bits and both wanted.  It was faster at every number of rows tried, 16 to 524288
@@ -459,12 +470,13 @@ template <typename T, typename GR, bool AC, bool BC, int OUT, int MASK, int ACT 
     if (G.act != ACT) { launch_tile<T, GR, AC, BC, OUT, MASK, ACT + 1>(st, G, num_cus); return; }
   }
   auto kern = k_tile<T, GR, AC, BC, OUT, MASK, ACT>;
-  constexpr int lds = 4 * (GR::BM * 64 + GR::BN * 64 + (MASK ? 1024 : 0));
+  constexpr int lds = GR::RING * (GR::BM * 64 + GR::BN * 64 + (MASK == 1 ? GR::BM * 4 : MASK == 2 ? GR::BN * 4 : 0)), slots_per_cu = 8 / GR::WAVES;
   nerfds::allow_dynamic_lds(reinterpret_cast<const void*>(kern), lds);
   G.tiles_n = (int)up(G.N, GR::BN);
   G.tiles = up(G.M, GR::BM) * G.tiles_n;
   const long long items = G.tiles * G.splits;
-  hipLaunchKernelGGL(kern, dim3((unsigned)(items < num_cus ? items : num_cus)), dim3(512), lds, st, G);
+  const long long slots = (long long)num_cus * slots_per_cu;
+  hipLaunchKernelGGL(kern, dim3((unsigned)(items < slots ? items : slots)), dim3(64 * GR::WAVES), lds, st, G);
 }
 
 constexpr int LDS_BYTES = 160 * 1024, RESIDENT_N = 256, RESIDENT_M = 16384;
@@ -491,6 +503,14 @@ template <typename T, bool AC, bool BC, int OUT, int MASK> void launch(hipStream
   if constexpr (sizeof(T) == 2) {
     // The large tiles pay where they fill the card; with fewer the 128 x 128 tiles below spread the work over more CUs
     if (tile_fits<AC, BC, MASK>(G) && (OUT == OUT_WEIGHTS || up(G.M, 256) * up(G.N, 128) >= num_cus / 2)) {
+      if constexpr (OUT != OUT_WEIGHTS) {
+        // Two workgroups per CU on half the tile where the whole ones leave CUs idle: 4096 x 1024 -> 1024 (64 tiles) 38 -> 29 us, 16384 x 512 -> 512 (128 tiles)
+        // 27 -> 22; 8192 x 4096 -> 2048 (256 tiles) would go from 136 to 141
+        if (G.N > 128 && up(G.M, 256) * up(G.N, 256) < num_cus) {
+          launch_tile<T, GridPair, AC, BC, OUT, MASK>(st, G, num_cus);
+          return;
+        }
+      }
       if (G.N > 128) launch_tile<T, Grid256, AC, BC, OUT, MASK>(st, G, num_cus);
       else launch_tile<T, Grid128, AC, BC, OUT, MASK>(st, G, num_cus);
       return;
@@ -534,14 +554,15 @@ template <typename T> void backward_t(hipStream_t st, const DenseBwd& w, int num
   char* ws = static_cast<char*>(w.ws);
   const void* dz = w.dy;
   long long lddz = w.lddy;
-  if (w.act != ACT_NONE && w.act != ACT_RELU) {
+  const bool stored = stores_dz(w);
+  if (stored) {
     const long long grans = w.m * up(w.n, 8), want = up(grans, 256);
-    hipLaunchKernelGGL((k_dz<T>), dim3((unsigned)(want < 16LL * num_cus ? want : 16LL * num_cus)), dim3(256), 0, st, static_cast<const T*>(w.dy), w.lddy,
-                       static_cast<const T*>(w.save), reinterpret_cast<T*>(ws), w.m, w.n, w.act);
+    hipLaunchKernelGGL((w.act == ACT_RELU ? k_dz<T, true> : k_dz<T, false>), dim3((unsigned)(want < 16LL * num_cus ? want : 16LL * num_cus)), dim3(256), 0, st,
+                       static_cast<const T*>(w.dy), w.lddy, w.save, reinterpret_cast<T*>(ws), w.m, w.n, w.act);
     dz = ws; lddz = w.n;
     ws += aligned((size_t)w.m * w.n * sizeof(T));
   }
-  const unsigned char* bits = w.act == ACT_RELU ? static_cast<const unsigned char*>(w.save) : nullptr;
+  const unsigned char* bits = w.act == ACT_RELU && !stored ? static_cast<const unsigned char*>(w.save) : nullptr;
   if constexpr (sizeof(T) == 2) {
     if (both_at_once(w)) {
       const int grid = weight_splits(w, num_cus).count;
@@ -584,7 +605,7 @@ size_t dense_save_bytes(int dtype, int act, long long m, int n) {
 }
 size_t dense_bwd_ws(const DenseBwd& a, int num_cus) {
   const Splits s = weight_splits(a, num_cus);
-  size_t b = a.act != ACT_NONE && a.act != ACT_RELU ? aligned((size_t)a.m * a.n * dtype_bytes(a.dtype)) : 0;
+  size_t b = stores_dz(a) ? aligned((size_t)a.m * a.n * dtype_bytes(a.dtype)) : 0;
   if (a.dkernel != nullptr || a.dbias != nullptr) b += weight_part_bytes(a, s.count) + aligned((size_t)s.count * up(a.n, 4) * 16);
   return b;
 }

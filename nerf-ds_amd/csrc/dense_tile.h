@@ -5,7 +5,8 @@
 // What bounds it and why these shapes: with k = n = 256 (a trunk layer) a byte of x is worth 256 multiply-adds, so the kernel has to stream; with
 // k, n in the thousands the matrix pipe is the bound and LDS next to it: a wave of 128 x 64 outputs reads 6 KiB of fragments for 8 MFMAs of 32 cycles, three
 // quarters of what LDS can give four SIMDs (64 x 64: all of it).  8 waves share a tile of 256 x 256 (or 256 x 128 where n is no more), one workgroup
-// per CU.
+// per CU; where those tiles are fewer than the CUs, two workgroups of 4 waves per CU share the card on 128 x 256.  8192 x 2048 -> 4096 in bf16: 139 us for the
+// product (989 TFLOP/s), 167 with bias, gelu, its saved input and the residual; dx 133, the weight gradient 151.
 #pragma once
 
 extern __shared__ __attribute__((aligned(16))) char g_lds[];
@@ -22,18 +23,18 @@ template <int N> OPS_DEV void wait_loads() { asm volatile("s_waitcnt vmcnt(%0) l
 //   contiguous: LDS row = line, 4 granules of 8 steps; strided: LDS row = step, LINES / 8 granules of 8 lines, read transposed.
 //   PERM: fragments take the lines of a 32-line tile with bits 2 and 3 of their number swapped, which leaves each lane of the accumulator 8 consecutive
 //   outputs at a time (first operand of the MFMA only).
-template <int LINES_, bool CONT_, bool PERM> struct Stage {
-  static constexpr int LINES = LINES_, BK = 32, BYTES = LINES * BK * 2, INSTR = BYTES / 1024, IPW = INSTR / 8;
+template <int LINES_, bool CONT_, bool PERM, int WAVES> struct Stage {
+  static constexpr int LINES = LINES_, BK = 32, BYTES = LINES * BK * 2, INSTR = BYTES / 1024, IPW = INSTR / WAVES;
   static constexpr bool CONT = CONT_;
   static constexpr int ROWG = CONT ? BK / 8 : LINES / 8;      // granules of an LDS row
-  static_assert(INSTR % 8 == 0, "whole instructions for 8 waves");
+  static_assert(INSTR % WAVES == 0, "whole instructions for each wave");
   static OPS_DEV int swz(int row) {
     // (16 lanes read together: 16 lines at one step, 4 to the 256 bytes that the banks span; or 4 steps of 4 granules)
     return CONT ? row >> 2 & 3 : (row & 3) << 2;
   }
   // this lane's granule of DMA instruction u of its wave
   static OPS_DEV void place(int u, int& row, int& g) {
-    const int slot = ((threadIdx.x >> 6) + 8 * u) * 64 + (threadIdx.x & 63);
+    const int slot = ((threadIdx.x >> 6) + WAVES * u) * 64 + (threadIdx.x & 63);
     row = slot / ROWG;
     g = (slot % ROWG) ^ swz(row);
   }
@@ -56,12 +57,13 @@ template <int LINES_, bool CONT_, bool PERM> struct Stage {
 };
 
 // WGM x WGN waves of (32 TM) x (32 TN) outputs
-template <int WGM_, int WGN_, int TM_, int TN_> struct Grid8 {
-  static constexpr int WGM = WGM_, WGN = WGN_, TM = TM_, TN = TN_, BM = 32 * WGM * TM, BN = 32 * WGN * TN;
-  static_assert(WGM * WGN == 8, "8 waves");
+template <int WGM_, int WGN_, int TM_, int TN_, int RING_> struct Grid {
+  static constexpr int WGM = WGM_, WGN = WGN_, TM = TM_, TN = TN_, BM = 32 * WGM * TM, BN = 32 * WGN * TN, WAVES = WGM * WGN, RING = RING_;
+  static_assert(WAVES == 8 || WAVES == 4, "two waves per SIMD: one workgroup per CU, or two");
 };
-typedef Grid8<2, 4, 4, 2> Grid256;      // 256 x 256
-typedef Grid8<4, 2, 2, 2> Grid128;      // 256 x 128
+typedef Grid<2, 4, 4, 2, 4> Grid256;      // 256 x 256
+typedef Grid<4, 2, 2, 2, 4> Grid128;      // 256 x 128
+typedef Grid<1, 4, 4, 2, 3> GridPair;     // 128 x 256, two workgroups per CU
 
 // Position in the order of work -> output tile: bands of 8 tile rows, down the band first, so that the tiles in flight on one XCD form a block and share
 // operand tiles both ways
@@ -72,12 +74,13 @@ OPS_DEV void tile_of(long long order, long long tiles_m, long long tiles_n, long
 }
 
 // MASK: 0, or the operand (1 = a, 2 = b) that is multiplied by the relu bits, in LDS, after its stage has landed
-template <typename T, typename GR, bool AC, bool BC, int OUT, int MASK, int ACT> __global__ __launch_bounds__(512) void k_tile(const GemmArgs G) {
-  typedef Stage<GR::BM, AC, false> SA;
-  typedef Stage<GR::BN, BC, true> SB;
-  constexpr int BK = 32, RING = 4, TM = GR::TM, TN = GR::TN;
-  constexpr int MB = MASK ? 1024 : 0, STAGE = SA::BYTES + SB::BYTES + MB, IPW = SA::IPW + SB::IPW + (MASK ? 1 : 0);
-  static_assert(!MASK || (MASK == 1 ? AC && GR::BM == 256 : !BC), "masked operand");
+template <typename T, typename GR, bool AC, bool BC, int OUT, int MASK, int ACT> __global__ __launch_bounds__(64 * GR::WAVES, 2) void k_tile(const GemmArgs G) {
+  typedef Stage<GR::BM, AC, false, GR::WAVES> SA;
+  typedef Stage<GR::BN, BC, true, GR::WAVES> SB;
+  constexpr int BK = 32, RING = GR::RING, WAVES = GR::WAVES, TM = GR::TM, TN = GR::TN;
+  constexpr int MW = MASK == 1 ? GR::BM / 64 : GR::BN / 64, MB = MASK ? MW * 256 : 0,      // DMA instructions and bytes of a stage's relu bits
+                STAGE = SA::BYTES + SB::BYTES + MB, IPW = SA::IPW + SB::IPW + (MASK ? 1 : 0);
+  static_assert(!MASK || ((MASK == 1 ? AC : !BC) && MW <= WAVES), "masked operand");
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / GR::WGN, wn = wave % GR::WGN;
   const unsigned lds0 = __builtin_amdgcn_readfirstlane((unsigned)(size_t)(__attribute__((address_space(3))) char*)g_lds);
   const char* const zeros = reinterpret_cast<const char*>(g_zeros);
@@ -124,14 +127,14 @@ template <typename T, typename GR, bool AC, bool BC, int OUT, int MASK, int ACT>
       okb[u] = line < G.N;
       pb[u] = static_cast<const char*>(G.b) + (BC ? line * G.ldb + c_i + cb[u] : (c_i + cb[u]) * G.ldb + line) * 2;
     }
-    if constexpr (MASK == 1) {      // 256 lines x 4 bytes: dword d of the block is line d; waves 4 - 7 fetch what waves 0 - 3 do, so that every wave counts alike
-      const long long line = m0 + 64 * (wave & 3) + lane;
+    if constexpr (MASK == 1) {      // BM lines x 4 bytes: dword d of the block is line d; waves past the last fetch the same again, so that every wave counts alike
+      const long long line = m0 + 64 * (wave & (MW - 1)) + lane;
       okm = line < G.M;
       pm = reinterpret_cast<const char*>(G.mask) + line * G.ldm + (c_i >> 3);
     }
     if constexpr (MASK == 2) {      // 32 steps x BN / 8 bytes
       constexpr int D = GR::BN / 32;
-      const int d = 64 * (wave & (GR::BN == 256 ? 3 : 1)) + lane;
+      const int d = 64 * (wave & (MW - 1)) + lane;
       cm = d / D;
       const long long line = n0 + 32 * (d % D);
       okm = line < G.N;
@@ -144,17 +147,16 @@ template <typename T, typename GR, bool AC, bool BC, int OUT, int MASK, int ACT>
     const unsigned base = lds0 + slot * STAGE;
 #pragma unroll
     for (int u = 0; u < SA::IPW; ++u) {
-      dma16(run && oka[u] && c_i + ca[u] < c1_i ? pa[u] : zeros, base + (wave + 8 * u) * 1024);
+      dma16(run && oka[u] && c_i + ca[u] < c1_i ? pa[u] : zeros, base + (wave + WAVES * u) * 1024);
       pa[u] += stepa;
     }
 #pragma unroll
     for (int u = 0; u < SB::IPW; ++u) {
-      dma16(run && okb[u] && c_i + cb[u] < c1_i ? pb[u] : zeros, base + SA::BYTES + (wave + 8 * u) * 1024);
+      dma16(run && okb[u] && c_i + cb[u] < c1_i ? pb[u] : zeros, base + SA::BYTES + (wave + WAVES * u) * 1024);
       pb[u] += stepb;
     }
     if constexpr (MASK != 0) {
-      const int w = MASK == 1 || GR::BN == 256 ? wave & 3 : wave & 1;
-      dma4(run && okm && c_i + cm < c1_i ? pm : zeros, base + SA::BYTES + SB::BYTES + w * 256);
+      dma4(run && okm && c_i + cm < c1_i ? pm : zeros, base + SA::BYTES + SB::BYTES + (wave & (MW - 1)) * 256);
       pm += MASK == 1 ? BK / 8 : BK * G.ldm;
     }
     c_i += BK;
@@ -191,7 +193,7 @@ template <typename T, typename GR, bool AC, bool BC, int OUT, int MASK, int ACT>
         for (int u = 0; u < SM::IPW; ++u) {
           int row, g;
           SM::place(u, row, g);
-          u32x4* at = reinterpret_cast<u32x4*>(op + ((wave + 8 * u) * 64 + lane) * 16);
+          u32x4* at = reinterpret_cast<u32x4*>(op + ((wave + WAVES * u) * 64 + lane) * 16);
           Gran<T> v{*at};
           gran_mask<T>(v, bits[row * SM::ROWG + g]);
           *at = v.v;

@@ -157,11 +157,26 @@ BOTH = [(32768, 256, 256, 'relu'), (150001, 256, 256, 'relu'), (140003, 160, 136
 @pytest.mark.parametrize('t', [F16, BF16], ids=['f16', 'bf16'])
 @pytest.mark.parametrize('i', range(len(BOTH)), ids=['%dx%dx%d-%s' % s for s in BOTH])
 def test_dense_gradients_of_narrow_layers(i, t):
-  m, k, n, act = BOTH[i]
+  _gradients_together_and_apart(*BOTH[i], t)
+
+
+# tiles that fill the card in each direction, relu with its bits tested in the tiles and before them
+WIDE = [(16645, 264, 1032, 'gelu'), (16645, 1040, 64, 'relu'), (16645, 520, 1056, 'relu'), (33000, 520, 512, 'relu'), (33001, 512, 544, 'relu'), (16645, 72, 1024, 'none'), (777, 1048, 1032, 'relu')]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('t', [F16, BF16], ids=['f16', 'bf16'])
+@pytest.mark.parametrize('i', range(len(WIDE)), ids=['%dx%dx%d-%s' % s for s in WIDE])
+def test_dense_wide_layers_over_many_rows(i, t):
+  _gradients_together_and_apart(*WIDE[i], t)
+
+
+def _gradients_together_and_apart(m, k, n, act, t):
   grid = 0.25 if act == 'relu' else None
   x, w, dy = dev(make(m, k, t=t, seed=6, grid=grid), make(k, n, t=t, seed=7, scale=1.0 if grid else k ** -0.5, grid=grid), make(m, n, t=t, seed=8))
   want = dense64(x, w, None, None, act, dy)
-  _, saved = layers.dense_forward(x, w, None, act)
+  y, saved = layers.dense_forward(x, w, None, act)
+  close(y, want['y'])
   first = layers.dense_backward(dy, x, w, saved, act)
   for name, g in zip(('dx', 'dkernel', 'db'), first):
     close(g, want[name], name)
