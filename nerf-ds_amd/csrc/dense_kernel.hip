@@ -29,6 +29,8 @@ struct GemmArgs {
   void* save; long long lds; int act;
   float* part; float* colpart; int splits; long long cps;      // weights: [splits][M][N], [splits][N], contraction per split (a multiple of BK)
   int tiles_n; long long tiles;
+  long long lo;      // k_gemm: elements from dz to its second part, 0: it has one (data: operand a, weights: operand b)
+  bool large;        // weights: k_tile takes it
 };
 
 template <typename T> struct Shape;
@@ -238,14 +240,17 @@ __global__ __launch_bounds__(THREADS, 2) void k_gemm(const GemmArgs G) {
   Gran<T> ra[TA::NG], rb[TB::NG];
   float cs[8] = {};
   const bool sums = OUT == OUT_WEIGHTS && G.colpart != nullptr && m0 == 0;
+  const T* pa = static_cast<const T*>(G.a);
+  const T* pb = static_cast<const T*>(G.b);
+  bool more = OUT != OUT_FORWARD && !MASK && sizeof(T) == 2 && G.lo != 0;
   auto fetch = [&](long long c) __attribute__((always_inline)) {
-    TA::load(ra, G.a, G.lda, m0, G.M, c, c1);
-    TB::load(rb, G.b, G.ldb, n0, G.N, c, c1);
+    TA::load(ra, pa, G.lda, m0, G.M, c, c1);
+    TB::load(rb, pb, G.ldb, n0, G.N, c, c1);
     if constexpr (MASK == 1) TA::mask(ra, G.mask, G.ldm, m0, G.M, c, c1);
     if constexpr (MASK == 2) TB::mask(rb, G.mask, G.ldm, n0, G.N, c, c1);
   };
   fetch(c0);
-  for (long long c = c0; c < c1; c += BK) {
+  for (long long c = c0; c < c1;) {
     __syncthreads();
     TA::stage(ra, lds);
     TB::stage(rb, lds + TA::BYTES);
@@ -258,7 +263,13 @@ __global__ __launch_bounds__(THREADS, 2) void k_gemm(const GemmArgs G) {
       }
     }
     __syncthreads();
-    if (c + BK < c1) fetch(c + BK);
+    c += BK;
+    if (c >= c1 && more) {      // the whole contraction again with the second part of dz
+      more = false;
+      c = c0;
+      (OUT == OUT_WEIGHTS ? pb : pa) += G.lo;
+    }
+    if (c < c1) fetch(c);
 #pragma unroll
     for (int ks = 0; ks < BK / 16; ++ks) {
       u32x4 fa[2][P], fb[2][P];
@@ -396,8 +407,9 @@ template <typename T, int M> __global__ __launch_bounds__(256) void k_rows(const
 }
 
 // dz = dy act'(z), once, for the activations whose slope costs more than a bit test (the products below read dz once per tile of their other axis), and for relu
-// (z: its bits) where those tiles are many.  dz is rounded to the tensors' type: the matrix pipe takes it in no other.
-template <typename T, bool RELU> __global__ __launch_bounds__(256) void k_dz(const T* __restrict__ dy, long long lddy, const void* __restrict__ z, T* __restrict__ dz, long long m, int n, int act) {
+// (z: its bits) where those tiles are many.  dz is rounded to the tensors' type: the matrix pipe takes it in no other.  Small layers (two_parts) get what
+// that rounding lost as a second array lo elements on.
+template <typename T, bool RELU> __global__ __launch_bounds__(256) void k_dz(const T* __restrict__ dy, long long lddy, const void* __restrict__ z, T* __restrict__ dz, long long m, int n, int act, long long lo) {
   const int gn = (n + 7) / 8;
   for (long long i = blockIdx.x * 256LL + threadIdx.x; i < m * gn; i += gridDim.x * 256LL) {
     const long long row = i / gn;
@@ -413,6 +425,14 @@ template <typename T, bool RELU> __global__ __launch_bounds__(256) void k_dz(con
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] *= gran_get<T>(a, j);
       a = gran_pack<T>(v);
+      if (lo != 0) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float high = gran_get<T>(a, j);
+          v[j] = fabsf(high) < __builtin_huge_valf() ? v[j] - high : 0.f;
+        }
+        gran_store<T>(dz + lo + row * n + c, gran_pack<T>(v), n - c);
+      }
     }
     gran_store<T>(dz + row * n + c, a, n - c);
   }
@@ -428,16 +448,26 @@ bool stores_dz(const DenseBwd& w) {
   if (w.act == ACT_NONE || w.act == ACT_RELU) return w.act == ACT_RELU && w.dtype != F32 && w.k > (w.dx && w.dkernel ? 512 : 1024) && w.k % 8 == 0 && w.n % 8 == 0 && whole_granules(w.x, w.ldx);
   return true;
 }
-// whether the weight gradient can go through k_tile: its operands' rows are whole, aligned granules, relu bits whole dwords (a dz in the workspace is)
-bool weight_tiles_large(const DenseBwd& w) {
-  if (w.dtype == F32 || w.k % 8 || w.n % 8 || !whole_granules(w.x, w.ldx)) return false;
+// Whether dz keeps its float32 value in two parts, which the products take one after the other: 16-bit layers so small that their time is latency, where the
+// rounding of dz would be the larger half of the gradients' error (45% more than the rounding of the results alone) and costs 1 - 4 us to avoid.
+bool two_parts(const DenseBwd& w) { return w.dtype != F32 && w.act != ACT_NONE && w.act != ACT_RELU && w.m <= 65536 / w.n; }
+// Whether the operands of the weight gradient suit the tiles that come by DMA: whole, aligned granules, relu bits in whole dwords (a dz in the workspace is)
+bool weight_dma(const DenseBwd& w) {
+  if (w.dtype == F32 || w.k % 8 || w.n % 8 || !whole_granules(w.x, w.ldx) || two_parts(w)) return false;
   if (stores_dz(w)) return true;
   return whole_granules(w.dy, w.lddy) && (w.act != ACT_RELU || (w.n % 32 == 0 && reinterpret_cast<uintptr_t>(w.save) % 4 == 0));
 }
+// Whether the weight gradient takes the large tiles: from 2^34 multiply-adds on, or where the rows are so many that memory is the bound.  (k_gemm has more
+// workgroups in flight, k_tile the higher rate: 512 x 512 in bf16 at 32768 rows 41 us by k_gemm and 44 by k_tile, at 65536 rows 68 and 60; 1024 x 1024 at 8192
+// rows 38 and 42, at 32768 rows 106 and 91; 256 x 256 at 4096 rows 13 and 21)
+bool weight_tiles_large(const DenseBwd& w) { return weight_dma(w) && (w.m >= 131072 || w.m >= (1LL << 34) / ((long long)w.k * w.n)); }
 
-// Whether both gradients come from one pass (k_both): a narrow layer in 16 bits and both wanted.  It was faster at every number of rows tried, 16 to 524288
-// (256 x 256 in bf16: 16 us instead of 10 + 11 at 16 rows, 28 instead of 9 + 26 at 4096, 213 instead of 119 + 130 at 524288).
-bool both_at_once(const DenseBwd& w) { return w.dx != nullptr && w.dkernel != nullptr && w.k <= 256 && w.n <= 256 && weight_tiles_large(w); }
+// Whether both gradients come from one pass (k_both): a narrow layer in 16 bits, both wanted.  Up to 128 x 256 at any number of rows (128 x 128 in bf16: 9.7 us
+// instead of 6.1 + 8.5 at 512 rows, 20.5 instead of 11 + 21 at 65536), the larger ones where their parts of dkernel have rows enough behind them (256 x 256: 32
+// instead of 8.5 + 17 at 8192 rows, 40 instead of 15 + 24 at 32768, 47 instead of 23 + 33 at 65536, 213 instead of 119 + 130 at 524288).
+bool both_at_once(const DenseBwd& w) {
+  return w.dx != nullptr && w.dkernel != nullptr && w.k <= 256 && w.n <= 256 && (w.k * w.n <= 128 * 256 || w.m >= 32768) && weight_dma(w);
+}
 
 struct Splits { int count; long long cps; };
 // The weight gradient has few output tiles (1 for 256 x 256) and a long contraction: as many splits as fill the card - one workgroup per CU of the large tiles,
@@ -456,13 +486,14 @@ Splits weight_splits(const DenseBwd& w, int num_cus) {
   return {(int)up(w.m, cps), cps};
 }
 
+size_t dz_bytes(const DenseBwd& w) { return stores_dz(w) ? aligned((size_t)up(w.m * w.n, 8) * 8 * dtype_bytes(w.dtype) * (two_parts(w) ? 2 : 1)) : 0; }
 size_t weight_part_bytes(const DenseBwd& w, int splits) {      // (one split of the weight gradient alone writes the result itself)
   return splits > 1 || both_at_once(w) ? aligned((size_t)splits * up((long long)w.k * w.n, 4) * 16) : 0;
 }
 
 // Whether k_tile can take the product: rows of whole, aligned granules on both sides (M, N and C too where they run along rows), relu bits in whole dwords
 template <bool AC, bool BC, int MASK> bool tile_fits(const GemmArgs& G) {
-  return whole_granules(G.a, G.lda) && whole_granules(G.b, G.ldb) && G.N % 8 == 0 && ((!AC && !BC) || G.C % 8 == 0) && (AC || G.M % 8 == 0) &&
+  return G.lo == 0 && whole_granules(G.a, G.lda) && whole_granules(G.b, G.ldb) && G.N % 8 == 0 && ((!AC && !BC) || G.C % 8 == 0) && (AC || G.M % 8 == 0) &&
          (!MASK || (G.ldm % 4 == 0 && reinterpret_cast<uintptr_t>(G.mask) % 4 == 0));
 }
 template <typename T, typename GR, bool AC, bool BC, int OUT, int MASK, int ACT = ACT_NONE> void launch_tile(hipStream_t st, GemmArgs& G, int num_cus) {
@@ -493,7 +524,7 @@ template <typename T, bool BC, int NP, int OUT, bool MASK, int ACT = ACT_NONE> v
 template <typename T, bool AC, bool BC, int OUT, int MASK> void launch(hipStream_t st, GemmArgs& G, int num_cus) {
   if constexpr (sizeof(T) == 2 && AC && OUT != OUT_WEIGHTS && MASK < 2) {
     // Many rows past a kernel that fits LDS.  RESIDENT_M: every workgroup fills 128 KiB of LDS first (3 us), which wants some 100 rows behind it
-    if (G.M >= RESIDENT_M && G.N <= RESIDENT_N && G.C <= 4096 && Resident::bytes((int)G.N, (int)G.C + (G.bias != nullptr)) <= LDS_BYTES) {
+    if (G.lo == 0 && G.M >= RESIDENT_M && G.N <= RESIDENT_N && G.C <= 4096 && Resident::bytes((int)G.N, (int)G.C + (G.bias != nullptr)) <= LDS_BYTES) {
       if (G.N <= 64) launch_resident<T, BC, 2, OUT, MASK == 1>(st, G, num_cus);
       else if (G.N <= 128) launch_resident<T, BC, 4, OUT, MASK == 1>(st, G, num_cus);
       else launch_resident<T, BC, 8, OUT, MASK == 1>(st, G, num_cus);
@@ -502,7 +533,7 @@ template <typename T, bool AC, bool BC, int OUT, int MASK> void launch(hipStream
   }
   if constexpr (sizeof(T) == 2) {
     // The large tiles pay where they fill the card; with fewer the 128 x 128 tiles below spread the work over more CUs
-    if (tile_fits<AC, BC, MASK>(G) && (OUT == OUT_WEIGHTS || up(G.M, 256) * up(G.N, 128) >= num_cus / 2)) {
+    if (tile_fits<AC, BC, MASK>(G) && (OUT == OUT_WEIGHTS ? G.large : up(G.M, 256) * up(G.N, 128) >= num_cus / 2)) {
       if constexpr (OUT != OUT_WEIGHTS) {
         // Two workgroups per CU on half the tile where the whole ones leave CUs idle: 4096 x 1024 -> 1024 (64 tiles) 38 -> 29 us, 16384 x 512 -> 512 (128 tiles)
         // 27 -> 22; 8192 x 4096 -> 2048 (256 tiles) would go from 136 to 141
@@ -555,12 +586,13 @@ template <typename T> void backward_t(hipStream_t st, const DenseBwd& w, int num
   const void* dz = w.dy;
   long long lddz = w.lddy;
   const bool stored = stores_dz(w);
+  const long long lo = two_parts(w) ? up(w.m * w.n, 8) * 8 : 0;
   if (stored) {
     const long long grans = w.m * up(w.n, 8), want = up(grans, 256);
     hipLaunchKernelGGL((w.act == ACT_RELU ? k_dz<T, true> : k_dz<T, false>), dim3((unsigned)(want < 16LL * num_cus ? want : 16LL * num_cus)), dim3(256), 0, st,
-                       static_cast<const T*>(w.dy), w.lddy, w.save, reinterpret_cast<T*>(ws), w.m, w.n, w.act);
+                       static_cast<const T*>(w.dy), w.lddy, w.save, reinterpret_cast<T*>(ws), w.m, w.n, w.act, lo);
     dz = ws; lddz = w.n;
-    ws += aligned((size_t)w.m * w.n * sizeof(T));
+    ws += dz_bytes(w);
   }
   const unsigned char* bits = w.act == ACT_RELU && !stored ? static_cast<const unsigned char*>(w.save) : nullptr;
   if constexpr (sizeof(T) == 2) {
@@ -578,7 +610,7 @@ template <typename T> void backward_t(hipStream_t st, const DenseBwd& w, int num
   if (w.dx != nullptr) {
     GemmArgs G{};
     G.a = dz; G.lda = lddz; G.b = w.kernel; G.ldb = w.ldk; G.M = w.m; G.N = w.k; G.C = w.n;
-    G.mask = bits; G.ldm = up(w.n, 8); G.y = w.dx; G.ldy = w.lddx; G.splits = 1; G.cps = w.n;
+    G.lo = lo; G.mask = bits; G.ldm = up(w.n, 8); G.y = w.dx; G.ldy = w.lddx; G.splits = 1; G.cps = w.n;
     if (bits) launch<T, true, true, OUT_PLAIN, 1>(st, G, num_cus); else launch<T, true, true, OUT_PLAIN, 0>(st, G, num_cus);
   }
   if (w.dkernel != nullptr || w.dbias != nullptr) {
@@ -586,7 +618,7 @@ template <typename T> void backward_t(hipStream_t st, const DenseBwd& w, int num
     GemmArgs G{};
     G.a = w.x; G.lda = w.ldx; G.b = dz; G.ldb = lddz; G.N = w.n; G.C = w.m;
     G.M = w.dkernel ? w.k : 1;      // (the bias gradient alone: it rides on the first tile of the kernel's rows)
-    G.mask = bits; G.ldm = up(w.n, 8); G.splits = s.count; G.cps = s.cps;
+    G.lo = lo; G.mask = bits; G.ldm = up(w.n, 8); G.splits = s.count; G.cps = s.cps; G.large = weight_tiles_large(w);
     const long long kn = (long long)w.k * w.n;
     const size_t part_bytes = weight_part_bytes(w, s.count);
     G.part = w.dkernel && s.count > 1 ? reinterpret_cast<float*>(ws) : nullptr;
@@ -605,7 +637,7 @@ size_t dense_save_bytes(int dtype, int act, long long m, int n) {
 }
 size_t dense_bwd_ws(const DenseBwd& a, int num_cus) {
   const Splits s = weight_splits(a, num_cus);
-  size_t b = stores_dz(a) ? aligned((size_t)a.m * a.n * dtype_bytes(a.dtype)) : 0;
+  size_t b = dz_bytes(a);
   if (a.dkernel != nullptr || a.dbias != nullptr) b += weight_part_bytes(a, s.count) + aligned((size_t)s.count * up(a.n, 4) * 16);
   return b;
 }

@@ -171,6 +171,27 @@ def test_dense_wide_layers_over_many_rows(i, t):
   _gradients_together_and_apart(*WIDE[i], t)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize('t', [F16, BF16], ids=['f16', 'bf16'])
+@pytest.mark.parametrize('act', ['sigmoid', 'softplus', 'silu', 'gelu'])
+def test_dense_small_gradients_lose_only_their_own_rounding(act, t):
+  for m, k, n in ((2, 438, 13), (17, 2, 32), (1, 40, 8), (200, 300, 256), (16500, 16, 3), (5, 7, 9001)):
+    # pre-activations that float32 sums exactly and the tensors' type holds, so that the saved ones are exact
+    x, w, b, dy = dev(make(m, k, t=t, seed=1, grid=1.0), make(k, n, t=t, seed=2, scale=0.5, grid=0.25), make(n, t=t, seed=3, grid=0.25), make(m, n, t=t, seed=4))
+    z = x.double() @ w.double() + b.double()
+    assert torch.equal(z.to(t).double(), z)
+    slope = act64(z, act)[1]
+    dz = dy.double() * slope
+    u = half_step(t)
+    # dz is not rounded: two parts keep u^2 of it (tiny: of a second part that underflows); beside that the slope's few float32 roundings, relative to 1
+    edz = 16 * E24 * dy.double().abs() + (u * u + 4 * E24) * dz.abs() + tiny(t)
+    _, saved = layers.dense_forward(x, w, b, act)
+    dx, dk, db = layers.dense_backward(dy, x, w, saved, act)
+    for got, v, e, length in ((dx, dz @ w.double().t(), edz @ w.double().abs().t(), n), (dk, x.double().t() @ dz, x.double().abs().t() @ edz, m), (db, dz.sum(0), edz.sum(0), m)):
+      total = dz.abs() @ w.double().abs().t() if got is dx else x.double().abs().t() @ dz.abs() if got is dk else dz.abs().sum(0)
+      close(got, (v, e + (length + 8) * E24 * total + u * v.abs() + tiny(t)), (m, k, n))
+
+
 def _gradients_together_and_apart(m, k, n, act, t):
   grid = 0.25 if act == 'relu' else None
   x, w, dy = dev(make(m, k, t=t, seed=6, grid=grid), make(k, n, t=t, seed=7, scale=1.0 if grid else k ** -0.5, grid=grid), make(m, n, t=t, seed=8))
