@@ -1,15 +1,17 @@
-// Both gradients of a narrow layer (k, n <= 256) over many rows from ONE read of x and dy: dx = dz kernel^T and dkernel = x^T dz.  Included by
+// Both gradients of a narrow layer (k, n <= 256) from ONE read of x and dy: dx = dz kernel^T and dkernel = x^T dz.  Included by
 // dense_kernel.hip only.
 //
 // What bounds it: memory (524288 x 256 x 256: 822 MB at the least; as two products dy is read twice, 1090 MB).  A persistent workgroup of 8 waves streams 32
-// rows of x and dy at a time through LDS by DMA, four such stages deep; the kernel stays in registers (64 per lane: each wave the 32 rows of it that make
-// its 32 columns of dx), and so does the workgroup's part of dkernel (128 per lane), written once at the end.  Per stage a wave does 32 MFMAs of 16
-// cycles for dx and 16 of 32 for dkernel: a third of the time that the stage's 50 KB take memory.
+// rows of x and dy at a time (16 where k and n are past 128) through LDS by DMA, four such stages deep.  The workgroup's part of dkernel stays in registers
+// (up to 128 per lane), written once at the end, and so does the kernel (each wave the 32 rows of it that make its 32 columns of dx); at 256 x 256 only three
+// eighths of it find room there, the rest waits in LDS, 80 KB of it (half in registers spilled).  For 16 rows of 256 x 256 a wave does 16 MFMAs of 16 cycles for
+// dx and 8 of 32 for dkernel: 0.4 us per CU with two waves on a SIMD, a third of the time that the rows' 25 KB take memory.
+// Measured: 197 - 235 us by the card, and 12 to add the 256 parts of dkernel (memory's floor 174; apart 119 - 128 and 130 - 142).
 #pragma once
 
 template <int KP_, int NP_> struct Both {
   static constexpr int KP = KP_, NP = NP_;      // k and n, padded to 128 or 256
-  // rows per stage: 32, or 16 for the layer of 256 x 256, where half the kernel waits in LDS (KL contraction steps; KR are in registers)
+  // rows per stage: 32, or 16 for the layer of 256 x 256, where KL of its contraction steps of 32 wait in LDS (KR are in registers)
   static constexpr bool FULL = KP == 256 && NP == 256;
   static constexpr int ROWS = FULL ? 16 : 32, XB = ROWS * KP * 2, YB = ROWS * NP * 2, BITS = ROWS * NP / 8, STAGE = XB + YB + BITS, RING = 4;
   static constexpr int KS = NP / 32, KL = FULL ? 5 : 0, KR = KS - KL, LDS = RING * STAGE + 8 * 2 * KL * 1024;

@@ -5,6 +5,7 @@
 // the time).  So everything serves loads in flight: a wave works alone on 16 rows at a time - no barrier after the kernel is in LDS -, its rows come straight
 // into registers in the layout the MFMA wants (16 rows x 64 contiguous bytes per load instruction), the next ones while it multiplies, and the residual of
 // the rows in hand as well: 64 KiB of x and as much of the residual under way per CU.  LDS gives the kernel's fragments once per 16 rows, a third of its time.
+// 524288 x 256 -> 256 in bf16 with bias, relu, its bits and the residual: 211 us (822 MB, 3.9 TB/s; a copy reaches 4.7); the data gradient alone 119 - 128.
 // Loads return in order, so nothing small may be asked for behind the next rows and waited for: the bias is one more contraction step of the kernel in LDS,
 // against a 1 behind the end of each row.
 #pragma once

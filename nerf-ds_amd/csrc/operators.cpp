@@ -1,5 +1,5 @@
 // C ABI of the stand-alone operators (include/nerfds.h): argument checks, the device, the launch.  No C++ exception leaves: messages are formatted
-// into a fixed buffer and everything below is free of allocation but the batch lists of ortho_kernel.hip, which live on the stack.
+// into a fixed buffer, the batch lists of ortho_kernel.hip live on the stack, and the one temporary of its sort is asked for without throwing.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdarg.h>

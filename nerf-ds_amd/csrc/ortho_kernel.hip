@@ -8,6 +8,10 @@
 // a product: measured against 64 bits it is as exact as float32 products (6e-7 after five steps at 256 x 256), at three times their rate.  One f16 plane
 // alone costs 2e-3 ... 5e-3, more than a bf16 result may be off.
 //
+// Measured: 256 x 256 and smaller, the 40 kernels of the field in float32: norm 9, preparation 15, then per step 9 + 8 + 14 us for the three products, each of which waits
+// for memory once or twice, not for its arithmetic; three of 1024 x 4096 and one of 2000 x 2047 in bf16: 20, 40 and 112 + 62 + 176 (UPDATE: 126 GFLOP of products of planes,
+// 716 TFLOP/s; GRAM waits for its longest contraction, 4096, in a single round of workgroups).
+//
 // Three ways through the same arithmetic, by size:
 //   whole   short side <= 64, long side <= 384: ONE workgroup takes the matrix through all steps in LDS (64 x 64: one launch, against 17)
 //   64      tiles of 64 x 64, one launch per product over all such matrices: bound by latency (a product of 256 x 256 is 10 - 16 workgroups of 4 steps)
@@ -40,7 +44,7 @@ struct Mat {
   long long ws;             // byte offset of its workspace
   int rows, cols;
 };
-struct Batch { char* ws; int tile, pad; int first[MAX_BATCH]; Mat m[MAX_BATCH]; };      // first: the matrix's first workgroup in this launch (unused entries: INT_MAX)
+struct Batch { char* ws; int tile; int first[MAX_BATCH]; Mat m[MAX_BATCH]; };      // first: the matrix's first workgroup in this launch (unused entries: INT_MAX)
 static_assert(sizeof(Batch) <= 4096, "kernel arguments");
 
 // workspace of one matrix: planes of X and of its transpose, twice (read one, write the other), of A and B, and the partial sums of the norm
@@ -196,8 +200,9 @@ extern __shared__ __attribute__((aligned(16))) char g_lds[];
 template <int N> OPS_DEV void wait_loads() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory"); }
 
 // One TS x TS tile of a product; GRAM and POLY are symmetric: tiles i <= j only, written twice.  Operand tiles arrive by LDS-DMA, 128 KiB of them under way
-// or in use (128-byte rows: a request then is a whole cache line, half as many as with rows of 64), one barrier a stage.  8 waves: four of (TS / 2) x (TS / 2) take the even, four the odd contraction steps of 16, and their sums are added - two waves
-// per SIMD, so that one's LDS reads run under the other's MFMAs, without reading any fragment more often.
+// or in use (128-byte rows: a request then is a whole cache line, half as many as with rows of 64; updates of 1024-wide matrices 183 -> 173 us), one barrier a stage.
+// 8 waves: four of (TS / 2) x (TS / 2) take the even, four the odd contraction steps of 16, and their sums are added - two waves per SIMD, so that one's LDS reads
+// run under the other's MFMAs, without reading any fragment more often.
 template <int TS> struct Ring {
   static constexpr int BK = 64, PLANE = TS * BK * 2, STAGE = 4 * PLANE, COUNT = TS == 64 ? 4 : 2, IPW = STAGE / 1024 / 8, EACH = IPW / 4;      // DMA instructions per wave: of a stage, of a plane
   // afterwards: the tile in float32, and its two planes transposed (rows padded against bank conflicts)

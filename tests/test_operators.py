@@ -689,7 +689,7 @@ def test_trainer_with_orthogonalised_kernels(nesterov):
       assert float((ema[off:off + rows * cols].double().reshape(rows, cols) - m[n]).abs().max()) <= 4 * E24 * float(m[n].abs().max())
       rest[off:off + rows * cols] = False
     # the other leaves: Adam's formula in another kernel, whose multiply-adds may be fused elsewhere: per step the moments differ by 2 roundings each, quotient,
-    # root and product by 4 more, the update (at most lr / sqrt(1 - b2) / ... = 3.2 lr in three steps) by 8 x 2^-24 of itself, the parameter by one
+    # root and product by 4 more, the update (at most 0.1 / sqrt(0.001) = 3.2 lr, the first step's bias correction aside, which makes it lr) by 8 x 2^-24 of itself, the parameter by one
     assert float((got[rest] - ref[rest]).abs().max()) <= (step + 1) * E24 * (8 * 3.2 * lr + float(ref[rest].abs().max()))
   assert muon.optimizer_step == 3 and not muon.nonfinite()
   before, moments = muon._download(0), muon._download(2)
