@@ -476,7 +476,7 @@ const char* nerfds_trainer_last_error(const nerfds_trainer* t);
  * bit per element for relu, the pre-activation in the element type for the smooth activations, nothing for none. */
 typedef struct nerfds_dense_forward_args {
   int32_t dtype, activation;
-  int64_t m;                          /* rows; 0 = nothing to do */
+  int64_t m;                          /* rows; 0 = nothing to do; fewer than 2^24 tiles of 128 x 128 in any of [m][k], [m][n], [k][n] */
   int32_t k, n;                       /* in, out; >= 1 */
   const void* x; int64_t ldx;         /* [m][k] */
   const void* kernel; int64_t ldk;    /* [k][n] */

@@ -71,7 +71,8 @@ int check_dense(const char* who, int32_t dtype, int32_t act, int64_t m, int32_t 
   if (act < 0 || act >= ACT_COUNT) return fail(NERFDS_EINVAL, "%s: unknown activation %d", who, act);
   if (m < 0 || m > MAX_ROWS || k < 1 || n < 1 || k > MAX_WIDTH || n > MAX_WIDTH)
     return fail(NERFDS_EINVAL, "%s: m = %lld, k = %d, n = %d (0 <= m <= 2^40, 1 <= k, n <= 2^24)", who, (long long)m, k, n);
-  if (tiles(m, n) >= (1LL << 31) || tiles(m, k) >= (1LL << 31) || tiles(k, n) >= (1LL << 31)) return fail(NERFDS_EINVAL, "%s: more than 2^31 output tiles", who);
+  // (a launch has less than 2^32 threads, a workgroup 256)
+  if (tiles(m, n) >= (1LL << 24) || tiles(m, k) >= (1LL << 24) || tiles(k, n) >= (1LL << 24)) return fail(NERFDS_EINVAL, "%s: 2^24 output tiles of 128 x 128 or more", who);
   return NERFDS_OK;
 }
 int check_array(const char* who, const char* name, const void* p, int32_t dtype, int64_t ld, int64_t least) {

@@ -643,6 +643,44 @@ def test_c_refusals():
   assert lib.nerfds_dense_forward(1000, C.byref(a), None) == EDEVICE and lib.nerfds_dense_forward(-1, C.byref(a), None) == EDEVICE
 
 
+def test_c_refuses_more_tiles_than_a_launch_holds():
+  lib = N.load()
+  p = 1 << 20      # never reached: refused on the host, on a machine with a GPU too
+  for m, k, n in ((1 << 33, 4, 128), (1 << 33, 128, 4), (1 << 31, 1, 1), (4, 1 << 21, 1 << 19)):
+    f = N.DenseForwardArgs(0, 0, m, k, n, p, k, p, n, None, None, 0, p, n, None)
+    b = N.DenseBackwardArgs(0, 0, m, k, n, p, k, p, n, p, n, None, p, k, p, p, p, 1 << 20)
+    assert lib.nerfds_dense_forward(0, C.byref(f), None) == -22 and lib.nerfds_dense_backward(0, C.byref(b), None) == -22
+    assert b'tiles' in lib.nerfds_last_error(None)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('t', [F32, F16, BF16], ids=['f32', 'f16', 'bf16'])
+def test_c_results_in_place(t):
+  lib, code, dev_ = N.load(), N.dtype_code(t), torch.cuda.current_device()
+  st = torch.cuda.current_stream().cuda_stream
+  for m, k, n, act in ((1, 256, 256, 'relu'), (7, 33, 65, 'gelu'), (300, 64, 100, 'silu'), (20003, 64, 200, 'relu'), (4100, 520, 1056, 'relu')):
+    x, w, b, r = dev(make(m, k, t=t, seed=1), make(k, n, t=t, seed=2, scale=k ** -0.5), make(n, t=t, seed=3), make(m, n, t=t, seed=4))
+    want, saved = layers.dense_forward(x, w, b, act, r)
+    save = torch.empty_like(saved)
+    a = N.DenseForwardArgs(code, N.ACTIVATIONS[act], m, k, n, x.data_ptr(), k, w.data_ptr(), n, b.data_ptr(), r.data_ptr(), n, r.data_ptr(), n, save.data_ptr())
+    assert lib.nerfds_dense_forward(dev_, C.byref(a), st) == 0
+    assert torch.equal(r, want) and torch.equal(save, saved), (m, k, n)      # y == residual
+  for m, d in ((5, 100), (33, 300), (9, 3000), (3, 9001)):
+    x, s = dev(make(m, d, t=t, seed=5), make(d, t=t, seed=6))
+    want = layers.layer_norm_forward(x, s)[0]
+    a = N.LayerNormForwardArgs(code, d, m, 1e-6, x.data_ptr(), d, s.data_ptr(), None, x.data_ptr(), d, None)
+    assert lib.nerfds_layer_norm_forward(dev_, C.byref(a), st) == 0
+    assert torch.equal(x, want), (m, d)
+  for shapes in ([(64, 64)], [(40, 130), (130, 40)], [(300, 200), (64, 64)], [(2000, 2047), (1100, 1000)]):
+    us = dev(*(make(r, c, t=t, seed=7 + i) for i, (r, c) in enumerate(shapes)))
+    want = optim.orthogonalize(us)
+    mats = (N.Matrix * len(us))(*(N.Matrix(u.data_ptr(), u.shape[1], u.data_ptr(), u.shape[1], *u.shape) for u in us))
+    nbytes = lib.nerfds_orthogonalize_workspace(mats, len(us))
+    ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device='cuda')
+    assert lib.nerfds_orthogonalize(dev_, code, mats, len(us), 5, ws.data_ptr(), nbytes, st) == 0
+    assert all(torch.equal(u, o) for u, o in zip(us, want)), shapes
+
+
 def test_struct_sizes_of_the_operators():
   lib = N.load()
   for which, st in ((9, N.DenseForwardArgs), (10, N.DenseBackwardArgs), (11, N.LayerNormForwardArgs), (12, N.LayerNormBackwardArgs), (13, N.Matrix)):
