@@ -5,7 +5,7 @@
 //                                                                                      kinds of leaves follow one learning-rate schedule
 //              flax.optim.Adam's                                                       on all others
 // One workgroup per 1024 elements of one leaf (a table made once); both do nothing where the gradient check of the step has raised its flag.  Bound by memory
-// and, at the 1.5 million parameters of the field (6 MB a vector), by the launch: 7 and 5 us around the 179 of the 40 orthogonalisations.
+// and, at the 1.5 million parameters of the field (6 MB a vector), by the launch: 7 and 5 us around the 160 of the 40 orthogonalisations.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 

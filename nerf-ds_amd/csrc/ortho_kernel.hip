@@ -8,7 +8,7 @@
 // a product: measured against 64 bits it is as exact as float32 products (6e-7 after five steps at 256 x 256), at three times their rate.  One f16 plane
 // alone costs 2e-3 ... 5e-3, more than a bf16 result may be off.
 //
-// Measured: 256 x 256 and smaller, the 40 kernels of the field in float32: norm 9, preparation 15, then per step 9 + 8 + 14 us for the three products, each of which waits
+// Measured: 256 x 256 and smaller, the 40 kernels of the field in float32: norm 9, preparation 15, then per step 9 + 8 + 12 us for the three products, each of which waits
 // for memory once or twice, not for its arithmetic; three of 1024 x 4096 and one of 2000 x 2047 in bf16: 20, 40 and 112 + 62 + 176 (UPDATE: 126 GFLOP of products of planes,
 // 716 TFLOP/s; GRAM waits for its longest contraction, 4096, in a single round of workgroups).
 //
@@ -32,6 +32,7 @@ namespace nerfds_ops {
 namespace {
 
 constexpr int THREADS = 256, WAVES8 = 512, TILE = 64, MAX_BATCH = 64;      // threads of the norm and the preparation, of the products
+constexpr unsigned CUS = 256;                           // of the card
 constexpr int WHOLE_N = 64, WHOLE_M = 384;             // sides of a matrix that one workgroup takes whole
 constexpr int SUM_ELEMS = 8192;                         // elements of U per workgroup of the norm, at the most
 constexpr float CA = 3.4445f, CB = -4.7750f, CC = 2.0315f;
@@ -199,19 +200,19 @@ extern __shared__ __attribute__((aligned(16))) char g_lds[];
 // all but the newest N loads have arrived, and this wave's LDS reads too: past the barrier that follows, the stage they came from may be overwritten
 template <int N> OPS_DEV void wait_loads() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory"); }
 
-// One TS x TS tile of a product; GRAM and POLY are symmetric: tiles i <= j only, written twice.  Operand tiles arrive by LDS-DMA, 128 KiB of them under way
+// One TS x TS tile of a product; GRAM and POLY are symmetric: tiles i <= j only, written twice.  Operand tiles arrive by LDS-DMA, up to 128 KiB of them under way
 // or in use (128-byte rows: a request then is a whole cache line, half as many as with rows of 64; updates of 1024-wide matrices 183 -> 173 us), one barrier a stage.
 // 8 waves: four of (TS / 2) x (TS / 2) take the even, four the odd contraction steps of 16, and their sums are added - two waves per SIMD, so that one's LDS reads
 // run under the other's MFMAs, without reading any fragment more often.
-template <int TS> struct Ring {
-  static constexpr int BK = 64, PLANE = TS * BK * 2, STAGE = 4 * PLANE, COUNT = TS == 64 ? 4 : 2, IPW = STAGE / 1024 / 8, EACH = IPW / 4;      // DMA instructions per wave: of a stage, of a plane
+template <int TS, int COUNT_> struct Ring {
+  static constexpr int BK = 64, PLANE = TS * BK * 2, STAGE = 4 * PLANE, COUNT = COUNT_, IPW = STAGE / 1024 / 8, EACH = IPW / 4;      // DMA instructions per wave: of a stage, of a plane
   // afterwards: the tile in float32, and its two planes transposed (rows padded against bank conflicts)
   static constexpr int ROWF = TS + 4, ROWT = TS + 8, OUTF = TS * ROWF * 4, OUTT = TS * ROWT * 2;
   static constexpr int LDS = COUNT * STAGE > OUTF + 2 * OUTT ? COUNT * STAGE : OUTF + 2 * OUTT;
   static_assert(IPW == 4 * EACH, "whole instructions per wave and plane");
 };
-template <int STEP, typename T, int TS> __global__ __launch_bounds__(WAVES8) void k_product(const Batch B, int cur) {
-  typedef Ring<TS> R;
+template <int STEP, typename T, int TS, int COUNT> __global__ __launch_bounds__(WAVES8) void k_product(const Batch B, int cur) {
+  typedef Ring<TS, COUNT> R;
   constexpr int BK = R::BK, W = TS / 64;      // 32 x 32 tiles per wave and side
   constexpr bool SYM = STEP == GRAM || STEP == POLY;
   constexpr int ROWB = BK * 2;
@@ -548,18 +549,24 @@ struct Ways {
       whole = whole && n <= WHOLE_N && m <= WHOLE_M;
       if (n >= 256) tiles += ((n + 127) / 128) * (long long)((m + 127) / 128);
     }
-    large = tiles >= 512;
+    large = tiles >= 2 * CUS;
   }
   Way of(const OrthoMat& m) const { return whole ? WHOLE : large && std::min(m.rows, m.cols) >= 256 ? TILES_128 : TILES_64; }
 };
 Layout layout_of(const OrthoMat& m, Way w) { return Layout(m.rows, m.cols, w == TILES_128 ? 128 : TILE); }
 
+template <int STEP, typename T, int TS, int COUNT> void product_of(hipStream_t st, dim3 grid, const Batch& B, int cur) {
+  typedef Ring<TS, COUNT> R;
+  nerfds::allow_dynamic_lds(reinterpret_cast<const void*>(&k_product<STEP, T, TS, COUNT>), R::LDS);
+  hipLaunchKernelGGL((k_product<STEP, T, TS, COUNT>), grid, dim3(WAVES8), R::LDS, st, B, cur);
+}
+// 64 x 64 tiles: four stages of 32 KiB, or two where the launch has more workgroups than the card has CUs, so that two of them share one (20 matrices of
+// 256 x 256: 148 us instead of 165; one of them 97 instead of 93, 768 x 3000 368 instead of 319).  128 x 128 tiles: two stages fill LDS as they are.
+template <int STEP, typename T, int TS> void product(hipStream_t st, dim3 grid, const Batch& B, int cur) {
+  if (TS == 128 || grid.x > CUS) product_of<STEP, T, TS, 2>(st, grid, B, cur); else product_of<STEP, T, TS, TS == 128 ? 2 : 4>(st, grid, B, cur);
+}
+
 template <typename T, int TS> void products(hipStream_t st, Batch& B, int count, int steps) {
-  typedef Ring<TS> R;
-  nerfds::allow_dynamic_lds(reinterpret_cast<const void*>(&k_product<GRAM, T, TS>), R::LDS);
-  nerfds::allow_dynamic_lds(reinterpret_cast<const void*>(&k_product<POLY, T, TS>), R::LDS);
-  nerfds::allow_dynamic_lds(reinterpret_cast<const void*>(&k_product<UPDATE, T, TS>), R::LDS);
-  nerfds::allow_dynamic_lds(reinterpret_cast<const void*>(&k_product<UPDATE_OUT, T, TS>), R::LDS);
   // workgroups of a launch: f(layout) per matrix
   auto spread = [&](auto f) {
     int total = 0;
@@ -568,18 +575,17 @@ template <typename T, int TS> void products(hipStream_t st, Batch& B, int count,
   };
   auto full = [](const Layout& L) { return (L.np / TS) * (L.mp / TS); };
   auto sym = [](const Layout& L) { const int t = L.np / TS; return t * (t + 1) / 2; };
-  const dim3 block(THREADS), block8(WAVES8);
+  const dim3 block(THREADS);
   dim3 grid = spread([](const Layout& L) { return L.sums; });
   hipLaunchKernelGGL((k_sumsq<T>), grid, block, 0, st, B);
   grid = spread([](const Layout& L) { return (L.np / TILE) * (L.mp / TILE); });
   hipLaunchKernelGGL((k_prepare<T>), grid, block, 0, st, B);
   for (int s = 0; s < steps; ++s) {
     grid = spread(sym);
-    hipLaunchKernelGGL((k_product<GRAM, T, TS>), grid, block8, R::LDS, st, B, s & 1);
-    hipLaunchKernelGGL((k_product<POLY, T, TS>), grid, block8, R::LDS, st, B, s & 1);
+    product<GRAM, T, TS>(st, grid, B, s & 1);
+    product<POLY, T, TS>(st, grid, B, s & 1);
     grid = spread(full);
-    if (s + 1 < steps) hipLaunchKernelGGL((k_product<UPDATE, T, TS>), grid, block8, R::LDS, st, B, s & 1);
-    else hipLaunchKernelGGL((k_product<UPDATE_OUT, T, TS>), grid, block8, R::LDS, st, B, s & 1);
+    if (s + 1 < steps) product<UPDATE, T, TS>(st, grid, B, s & 1); else product<UPDATE_OUT, T, TS>(st, grid, B, s & 1);
   }
 }
 
