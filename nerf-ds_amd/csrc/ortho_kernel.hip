@@ -411,7 +411,7 @@ template <typename T> __global__ __launch_bounds__(WAVES8) void k_whole(const Ba
   char* X = g_lds;                              // [2][64][mp]
   char* A = g_lds + 2 * xplane;
   char* P = A + 2 * 8192;
-  f32x4* even = reinterpret_cast<f32x4*>(P + 2 * 8192);      // [4 waves][4 quads][64 lanes]: the even steps' sums of a symmetric product
+  f32x4* sums = reinterpret_cast<f32x4*>(P + 2 * 8192);      // [4 tiles][4 quads][64 lanes]: what two waves of a tile give each other
   // X is read along its rows (16 lines, one granule) and across them (4 rows, 4 granules, transposed): the swizzle sends both to the 16 granules that the banks
   // span, in rows of 128 bytes (modulo 256) and of 256
   auto turn8 = [](int r) __attribute__((always_inline)) { return (r << 1 & 4) | (r >> 2 & 3); };
@@ -451,52 +451,70 @@ template <typename T> __global__ __launch_bounds__(WAVES8) void k_whole(const Ba
     const u32x2 b = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(base + xat(row + 4, g) + (i & 1) * 8)));
     return u32x4{a[0], a[1], b[0], b[1]};
   };
-  const int wi = wave >> 1 & 1, wj = wave & 1, odd = wave >> 2;      // as in k_product: even and odd contraction steps of 16
+  // GRAM: A = X X^T; POLY: P = b A + c A A; UPDATE: X <- a X + P X (in place: X is read by all before it is written).  Waves (wi, wj) have the 32 x 32
+  // tile (wi, wj), one the even and one the odd contraction steps of 16 as in k_product; each gives the other half of its sums and finishes the other half
+  // (64 x 64, one call: 23 us; 29 where the odd wave finishes all and two waves of eight make the update).
+  const int wi = wave >> 1 & 1, wj = wave & 1, odd = wave >> 2;
+  f32x4* const box = sums + (wave & 3) * 256 + lane;
   for (int step = 0; step < steps; ++step) {
 #pragma unroll
-    for (int kind = 0; kind < 2; ++kind) {      // GRAM: A = X X^T; POLY: P = b A + c A A: waves (wi, wj) have the 32 x 32 tile (wi, wj)
+    for (int kind = GRAM; kind <= UPDATE; ++kind) {
+      if (kind == UPDATE && L.mp > 64) break;
       f32x16 acc = {};
-      const int K = kind == 0 ? L.mp : WHOLE_N;
+      const int K = kind == GRAM ? L.mp : WHOLE_N;
 #pragma unroll 4
       for (int ks = odd; ks < K / 16; ks += 2) {
         u32x4 l[2], r[2];
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
-          l[p] = kind == 0 ? along(X + p * xplane, xat, wi, ks) : along(A + p * 8192, aat, wi, ks);
-          r[p] = kind == 0 ? along(X + p * xplane, xat, wj, ks) : along(A + p * 8192, aat, wj, ks);
+          l[p] = kind == GRAM ? along(X + p * xplane, xat, wi, ks) : along((kind == POLY ? A : P) + p * 8192, aat, wi, ks);
+          r[p] = kind == GRAM ? along(X + p * xplane, xat, wj, ks) : kind == POLY ? along(A + p * 8192, aat, wj, ks) : across(X + p * xplane, wj, ks);
         }
         acc = mma16(r[1], l[0], acc);
         acc = mma16(r[0], l[1], acc);
         acc = mma16(r[0], l[0], acc);
       }
-      char* out = kind == 0 ? A : P;
-      f32x4* mine = even + (wave & 3) * 256 + lane;
-      if (!odd) {
+      f32x4 own[2];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) mine[64 * q] = f32x4{acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
+      for (int h = 0; h < 2; ++h) {
+        const f32x4 low = {acc[4 * h], acc[4 * h + 1], acc[4 * h + 2], acc[4 * h + 3]}, high = {acc[4 * h + 8], acc[4 * h + 9], acc[4 * h + 10], acc[4 * h + 11]};
+        own[h] = odd ? high : low;
+        box[64 * (2 * (1 - odd) + h)] = odd ? low : high;
       }
       __syncthreads();
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        if (!odd) break;
-        const f32x4 first = mine[64 * q];
-        const int at = aat(32 * wi + (lane & 31), 4 * wj + q) + 8 * (lane >> 5);
-        float v[4];
+      for (int h = 0; h < 2; ++h) {
+        const int q = 2 * odd + h, row = 32 * wi + (lane & 31), col = 32 * wj + 8 * q + 4 * (lane >> 5);
+        const f32x4 given = box[64 * q];
+        const int at = (kind == UPDATE ? xat(row, col >> 3) : aat(row, col >> 3)) + 8 * (lane >> 5);
+        char* const from = kind == UPDATE ? X : A;
+        const int plane = kind == UPDATE ? xplane : 8192;
         u32x2 oh = {}, ol = {};
-        if (kind == 1) { oh = *reinterpret_cast<const u32x2*>(A + at); ol = *reinterpret_cast<const u32x2*>(A + 8192 + at); }
+        if (kind != GRAM) { oh = *reinterpret_cast<const u32x2*>(from + at); ol = *reinterpret_cast<const u32x2*>(from + plane + at); }
+        float v[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float x = first[e] + acc[4 * q + e];
-          v[e] = kind == 0 ? gram_of(x) : poly_of(f16_of(oh, e) + f16_of(ol, e), x);
+          const float x = given[e] + own[h][e], o = f16_of(oh, e) + f16_of(ol, e);
+          v[e] = kind == GRAM ? gram_of(x) : kind == POLY ? poly_of(o, x) : update_of(o, x);
         }
-        u32x2 pack[2];
-        split4(v, pack);
-        *reinterpret_cast<u32x2*>(out + at) = pack[0];
-        *reinterpret_cast<u32x2*>(out + 8192 + at) = pack[1];
+        if (kind == UPDATE && step + 1 == steps) {
+          T* o = static_cast<T*>(M.o);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (row < L.n && col + e < L.m) o[tall ? (col + e) * M.ldo + row : row * M.ldo + col + e] = from_f32<T>(v[e] * (1.f / SX));
+        } else {
+          char* const out = kind == GRAM ? A : kind == POLY ? P : X;
+          u32x2 pack[2];
+          split4(v, pack);
+          *reinterpret_cast<u32x2*>(out + at) = pack[0];
+          *reinterpret_cast<u32x2*>(out + plane + at) = pack[1];
+        }
       }
       __syncthreads();
     }
-    // UPDATE: a wave takes 32 columns of X whole (both row tiles), reads them, and writes them back in place
+    if (L.mp == 64) continue;
+    // UPDATE of a longer X: a wave takes 32 columns whole (both row tiles), reads them, and writes them back in place (64 x 384: 70 us; 81 by the way above, which
+    // needs two barriers for each 64 columns)
     for (int t = wave; t < L.mp / 32; t += 8) {
       f32x16 acc[2][2] = {};      // [row tile][even, odd]
 #pragma unroll
