@@ -484,6 +484,7 @@ typedef struct nerfds_dense_forward_args {
   const void* residual; int64_t ldr;  /* [m][n] or NULL; ldr = 0: one row for all */
   void* y; int64_t ldy;               /* [m][n], must not overlap an input (the residual in place is allowed: y == residual, ldy == ldr) */
   void* save;
+  void* workspace; int64_t workspace_bytes;   /* >= nerfds_dense_forward_workspace(), 256-byte aligned; or NULL: few rows then take a long k in one stretch */
 } nerfds_dense_forward_args;
 /* dz = dy act'(z); dx = dz kernel^T, dkernel = x^T dz, dbias = column sums of dz; the gradient of the residual is dy itself.  dx / dkernel / dbias may
  * be NULL (not computed).  For 16-bit tensors dz is rounded to their type between the slope and the products; none and
@@ -502,6 +503,7 @@ typedef struct nerfds_dense_backward_args {
   void* workspace; int64_t workspace_bytes;   /* >= nerfds_dense_backward_workspace(), 256-byte aligned */
 } nerfds_dense_backward_args;
 int64_t nerfds_dense_save_bytes(int32_t dtype, int32_t activation, int64_t m, int32_t n);                    /* negative: invalid argument */
+int64_t nerfds_dense_forward_workspace(int device, const nerfds_dense_forward_args* args);                  /* bytes, 0 = none; the sizes and the type are read */
 int64_t nerfds_dense_backward_workspace(int device, const nerfds_dense_backward_args* args);                /* bytes; the workspace fields are not read */
 int nerfds_dense_forward(int device, const nerfds_dense_forward_args* args, void* hip_stream);
 int nerfds_dense_backward(int device, const nerfds_dense_backward_args* args, void* hip_stream);

@@ -4,7 +4,7 @@
 //   weights   dk [k x n] = x^T        . dz [m x n]           contraction over m, split over workgroups and summed in a second kernel
 // dz = dy act'(z).  Each operand is stored with the contraction either along its rows ("contiguous") or across them ("strided"); a strided tile is
 // transposed on its way from LDS to the registers (ds_read_b64_tr_b16), so no operand is ever transposed in memory.
-// k_gemm below takes everything; dense_resident.h, dense_tile.h and dense_backward.h the 16-bit products that stream past a small kernel, that are large, and both
+// k_gemm below takes everything (a few rows' long contraction in pieces that k_join adds); dense_resident.h, dense_tile.h and dense_backward.h the 16-bit products that stream past a small kernel, that are large, and both
 // gradients of a narrow layer.  65536 x 256 -> 256 in float32 with softplus: forward 71 us, dz 35, dx 59, the weight gradient 54 - 60 and its sum 7 (six products of
 // parts each, 52 GFLOP: 46 us at the rate of a large 16-bit product, 720 - 960 TFLOP/s reached).
 #include <hip/hip_runtime.h>
@@ -296,21 +296,21 @@ __global__ __launch_bounds__(THREADS, 2) void k_gemm(const GemmArgs G) {
     }
   }
 
-  if constexpr (OUT == OUT_WEIGHTS) {
-    if (G.part != nullptr) {
-      float* out = G.part + blockIdx.y * ((G.M * G.N + 3) & ~3LL);
+  if (G.part != nullptr) {
+    float* out = G.part + blockIdx.y * ((G.M * G.N + 3) & ~3LL);
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const long long n = n0 + 64 * wn + 32 * j + (lane & 31);
+      for (int j = 0; j < 2; ++j) {
+        const long long n = n0 + 64 * wn + 32 * j + (lane & 31);
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const long long m = m0 + 64 * wm + 32 * i + (r & 3) + 8 * (r >> 2) + 4 * (lane >> 5);
-            if (m < G.M && n < G.N) out[m * G.N + n] = acc[i][j][r];
-          }
+        for (int r = 0; r < 16; ++r) {
+          const long long m = m0 + 64 * wm + 32 * i + (r & 3) + 8 * (r >> 2) + 4 * (lane >> 5);
+          if (m < G.M && n < G.N) out[m * G.N + n] = acc[i][j][r];
         }
-    }
+      }
+  }
+  if constexpr (OUT == OUT_WEIGHTS) {
     if (sums) {      // thread t holds the sums of columns 8 (t & 15) .. over its rows: 16 threads per column group
       float* red = reinterpret_cast<float*>(lds);
       __syncthreads();
@@ -324,7 +324,7 @@ __global__ __launch_bounds__(THREADS, 2) void k_gemm(const GemmArgs G) {
       }
     }
   }
-  if (OUT != OUT_WEIGHTS || G.y != nullptr) {
+  if (G.part == nullptr && (OUT != OUT_WEIGHTS || G.y != nullptr)) {
     // the wave's 64 x 64 block through LDS, 32 rows at a time, so that every lane finishes 8 consecutive elements of a row
     float* buf = reinterpret_cast<float*>(lds) + wave * 32 * 68;
     const long long n = n0 + 64 * wn + 8 * (lane & 7), valid = G.N - n;
@@ -358,6 +358,28 @@ __global__ __launch_bounds__(THREADS, 2) void k_gemm(const GemmArgs G) {
       }
     }
   }
+}
+
+// The end of a product whose contraction was split: a thread adds the parts of 8 elements in their order
+template <typename T, int OUT> __global__ __launch_bounds__(256) void k_join(const GemmArgs G) {
+  const long long gn = (G.N + 7) / 8, stride = (G.M * G.N + 3) & ~3LL, i = blockIdx.x * 256LL + threadIdx.x;
+  if (i >= G.M * gn) return;
+  const long long m = i / gn, n = i % gn * 8, valid = G.N - n;
+  float v[8] = {};
+#pragma unroll 4
+  for (int p = 0; p < G.splits; ++p) {
+    const Gran<float> g = gran_load<float>(G.part + p * stride + m * G.N + n, valid);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] += gran_get<float>(g, j);
+  }
+  if constexpr (OUT == OUT_FORWARD) {
+    if (G.bias != nullptr) {
+      const Gran<T> g = gran_load<T>(static_cast<const T*>(G.bias) + n, valid);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] += gran_get<T>(g, j);
+    }
+    finish<T>(v, m, n, valid, G.act, G.save, G.lds, G.residual, G.ldr, G.y, G.ldy);
+  } else gran_store<T>(static_cast<T*>(G.y) + m * G.ldy + n, gran_pack<T>(v), valid);
 }
 
 #include "dense_tile.h"
@@ -472,6 +494,10 @@ bool both_at_once(const DenseBwd& w) {
   return w.dx != nullptr && w.dkernel != nullptr && w.k <= 256 && w.n <= 256 && (w.k * w.n <= 128 * 256 || w.m >= 32768) && weight_dma(w);
 }
 
+constexpr int RESIDENT_M = 16384;
+// The large tiles pay where they fill the card; with fewer the 128 x 128 tiles of k_gemm spread the work over more CUs
+bool large_tiles_fill(long long m, long long n, int num_cus) { return up(m, 256) * up(n, 128) >= num_cus / 2; }
+
 struct Splits { int count; long long cps; };
 // The weight gradient has few output tiles (1 for 256 x 256) and a long contraction: as many splits as fill the card - one workgroup per CU of the large tiles,
 // two of the small ones.  A fraction of a round more is no gain: splits are rounded down there.  Few rows are cut short too, for each split is one chain of loads
@@ -488,6 +514,23 @@ Splits weight_splits(const DenseBwd& w, int num_cus) {
   const long long cps = up(steps, want) * 64;
   return {(int)up(w.m, cps), cps};
 }
+
+// Few output tiles over a long contraction (few rows): the forward's and dx's products by k_gemm are split as well and joined by k_join, where the chain of steps
+// they save (a step of 64 elements takes about 1.1 us in 16 bits, 4 in float32, whatever else runs) is longer than the join, which grows with the tiles.  Pieces are
+// two steps and more, all parts within 32 MB.  Whole and split: 9 x 4096 -> 64 in bf16 130 and 14 us, in float32 295 and 19; 512 x 2048 -> 2048 (64 tiles) in bf16 36 and
+// 22, but from k = 768 19 and 21; in float32 118 and 39, from k = 256 26 and 21.
+Splits row_splits(int dtype, long long m, long long n, long long c, int num_cus) {
+  const long long step = dtype == F32 ? 32 : 64, tiles = up(m, BM) * up(n, BN);
+  if (m <= 8 || tiles >= num_cus || c < (dtype == F32 ? 128 + 2 * tiles : 256 + 12 * tiles)) return {1, c};
+  if (dtype != F32 && (m >= RESIDENT_M || large_tiles_fill(m, n, num_cus))) return {1, c};      // (other kernels' work, whole)
+  long long want = 2LL * num_cus / tiles;
+  if (want > (1 << 23) / (m * n)) want = (1 << 23) / (m * n);
+  if (want > c / (2 * step)) want = c / (2 * step);
+  if (want <= 1) return {1, c};
+  const long long cps = up(c, want * step) * step;
+  return {(int)up(c, cps), cps};
+}
+size_t row_part_bytes(const Splits& s, long long m, long long n) { return s.count > 1 ? aligned((size_t)s.count * up(m * n, 4) * 16) : 0; }
 
 size_t dz_bytes(const DenseBwd& w) { return stores_dz(w) ? aligned((size_t)up(w.m * w.n, 8) * 8 * dtype_bytes(w.dtype) * (two_parts(w) ? 2 : 1)) : 0; }
 size_t weight_part_bytes(const DenseBwd& w, int splits) {      // (one split of the weight gradient alone writes the result itself)
@@ -513,7 +556,7 @@ template <typename T, typename GR, bool AC, bool BC, int OUT, int MASK, int ACT 
   hipLaunchKernelGGL(kern, dim3((unsigned)(items < slots ? items : slots)), dim3(64 * GR::WAVES), lds, st, G);
 }
 
-constexpr int LDS_BYTES = 160 * 1024, RESIDENT_N = 256, RESIDENT_M = 16384;
+constexpr int LDS_BYTES = 160 * 1024, RESIDENT_N = 256;
 template <typename T, bool BC, int NP, int OUT, bool MASK, int ACT = ACT_NONE> void launch_resident(hipStream_t st, GemmArgs& G, int num_cus) {
   if constexpr (OUT == OUT_FORWARD && ACT + 1 < ACT_COUNT) {
     if (G.act != ACT) { launch_resident<T, BC, NP, OUT, MASK, ACT + 1>(st, G, num_cus); return; }
@@ -535,8 +578,7 @@ template <typename T, bool AC, bool BC, int OUT, int MASK> void launch(hipStream
     }
   }
   if constexpr (sizeof(T) == 2) {
-    // The large tiles pay where they fill the card; with fewer the 128 x 128 tiles below spread the work over more CUs
-    if (tile_fits<AC, BC, MASK>(G) && (OUT == OUT_WEIGHTS ? G.large : up(G.M, 256) * up(G.N, 128) >= num_cus / 2)) {
+    if (tile_fits<AC, BC, MASK>(G) && (OUT == OUT_WEIGHTS ? G.large : large_tiles_fill(G.M, G.N, num_cus))) {
       if constexpr (OUT != OUT_WEIGHTS) {
         // Two workgroups per CU on half the tile where the whole ones leave CUs idle: 4096 x 1024 -> 1024 (64 tiles) 38 -> 29 us, 16384 x 512 -> 512 (128 tiles)
         // 27 -> 22; 8192 x 4096 -> 2048 (256 tiles) would go from 136 to 141
@@ -553,6 +595,9 @@ template <typename T, bool AC, bool BC, int OUT, int MASK> void launch(hipStream
   G.tiles_n = (int)up(G.N, BN);
   G.tiles = up(G.M, BM) * G.tiles_n;
   hipLaunchKernelGGL((k_gemm<T, AC, BC, OUT, MASK>), dim3((unsigned)G.tiles, G.splits), dim3(THREADS), 0, st, G);
+  if constexpr (OUT != OUT_WEIGHTS) {
+    if (G.part != nullptr) hipLaunchKernelGGL((k_join<T, OUT>), dim3((unsigned)up(G.M * up(G.N, 8), 256)), dim3(256), 0, st, G);
+  }
 }
 
 template <typename T> void forward_t(hipStream_t st, const DenseFwd& f, int num_cus) {
@@ -568,7 +613,9 @@ template <typename T> void forward_t(hipStream_t st, const DenseFwd& f, int num_
   G.a = f.x; G.lda = f.ldx; G.b = f.kernel; G.ldb = f.ldk; G.M = f.m; G.N = f.n; G.C = f.k;
   G.bias = f.bias; G.residual = f.residual; G.ldr = f.ldr; G.y = f.y; G.ldy = f.ldy; G.act = f.act;
   G.save = f.save; G.lds = f.act == ACT_RELU ? up(f.n, 8) : f.n;
-  G.splits = 1; G.cps = f.k;
+  const Splits s = f.ws != nullptr ? row_splits(f.dtype, f.m, f.n, f.k, num_cus) : Splits{1, f.k};
+  G.splits = s.count; G.cps = s.cps;
+  if (s.count > 1) G.part = static_cast<float*>(f.ws);
   launch<T, true, false, OUT_FORWARD, 0>(st, G, num_cus);
 }
 
@@ -613,7 +660,10 @@ template <typename T> void backward_t(hipStream_t st, const DenseBwd& w, int num
   if (w.dx != nullptr) {
     GemmArgs G{};
     G.a = dz; G.lda = lddz; G.b = w.kernel; G.ldb = w.ldk; G.M = w.m; G.N = w.k; G.C = w.n;
-    G.lo = lo; G.mask = bits; G.ldm = up(w.n, 8); G.y = w.dx; G.ldy = w.lddx; G.splits = 1; G.cps = w.n;
+    G.lo = lo; G.mask = bits; G.ldm = up(w.n, 8); G.y = w.dx; G.ldy = w.lddx;
+    const Splits s = row_splits(w.dtype, w.m, w.k, w.n, num_cus);
+    G.splits = s.count; G.cps = s.cps;
+    if (s.count > 1) G.part = reinterpret_cast<float*>(ws);      // (joined before the weight gradient's parts come here)
     if (bits) launch<T, true, true, OUT_PLAIN, 1>(st, G, num_cus); else launch<T, true, true, OUT_PLAIN, 0>(st, G, num_cus);
   }
   if (w.dkernel != nullptr || w.dbias != nullptr) {
@@ -638,11 +688,12 @@ template <typename T> void backward_t(hipStream_t st, const DenseBwd& w, int num
 size_t dense_save_bytes(int dtype, int act, long long m, int n) {
   return act == ACT_NONE ? 0 : act == ACT_RELU ? (size_t)m * up(n, 8) : (size_t)m * n * dtype_bytes(dtype);
 }
+size_t dense_fwd_ws(const DenseFwd& a, int num_cus) { return row_part_bytes(row_splits(a.dtype, a.m, a.n, a.k, num_cus), a.m, a.n); }
 size_t dense_bwd_ws(const DenseBwd& a, int num_cus) {
   const Splits s = weight_splits(a, num_cus);
-  size_t b = dz_bytes(a);
-  if (a.dkernel != nullptr || a.dbias != nullptr) b += weight_part_bytes(a, s.count) + aligned((size_t)s.count * up(a.n, 4) * 16);
-  return b;
+  const size_t weights = a.dkernel != nullptr || a.dbias != nullptr ? weight_part_bytes(a, s.count) + aligned((size_t)s.count * up(a.n, 4) * 16) : 0;
+  const size_t rows = a.dx != nullptr && !both_at_once(a) ? row_part_bytes(row_splits(a.dtype, a.m, a.k, a.n, num_cus), a.m, a.k) : 0;
+  return dz_bytes(a) + (weights > rows ? weights : rows);
 }
 void dense_forward(hipStream_t st, const DenseFwd& a, int num_cus) {
   if (a.dtype == F32) forward_t<float>(st, a, num_cus);

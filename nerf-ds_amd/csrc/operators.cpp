@@ -89,6 +89,9 @@ int check_workspace(const char* who, const void* p, int64_t have, int64_t need) 
   return NERFDS_OK;
 }
 
+DenseFwd dense_fwd_of(const nerfds_dense_forward_args& a) {
+  return DenseFwd{a.dtype, a.activation, a.m, a.k, a.n, a.x, a.ldx, a.kernel, a.ldk, a.bias, a.residual, a.ldr, a.y, a.ldy, a.save, a.workspace};
+}
 DenseBwd dense_bwd_of(const nerfds_dense_backward_args& a) {
   return DenseBwd{a.dtype, a.activation, a.m, a.k, a.n, a.x, a.ldx, a.kernel, a.ldk, a.dy, a.lddy, a.save, a.dx, a.lddx, a.dkernel, a.dbias, a.workspace};
 }
@@ -116,6 +119,15 @@ int64_t nerfds_dense_save_bytes(int32_t dtype, int32_t activation, int64_t m, in
   return (int64_t)dense_save_bytes(dtype, activation, m, n);
 }
 
+int64_t nerfds_dense_forward_workspace(int device, const nerfds_dense_forward_args* a) {
+  const char* who = "nerfds_dense_forward_workspace";
+  if (!a) return fail(NERFDS_EINVAL, "%s: null argument", who);
+  CHECK(check_dense(who, a->dtype, a->activation, a->m, a->k, a->n));
+  const int cus = num_cus(device);
+  if (cus == 0) return fail(NERFDS_EDEVICE, "%s: no such HIP device %d", who, device);
+  return (int64_t)dense_fwd_ws(dense_fwd_of(*a), cus);
+}
+
 int nerfds_dense_forward(int device, const nerfds_dense_forward_args* a, void* hip_stream) {
   const char* who = "nerfds_dense_forward";
   if (!a) return fail(NERFDS_EINVAL, "%s: null argument", who);
@@ -128,8 +140,9 @@ int nerfds_dense_forward(int device, const nerfds_dense_forward_args* a, void* h
   if (a->residual) CHECK(check_array(who, "residual", a->residual, a->dtype, a->ldr == 0 ? a->n : a->ldr, a->n));
   CHECK(check_vector(who, "save", a->save, a->activation == ACT_RELU ? F16 : a->dtype));
   ON_DEVICE(who, device);
-  dense_forward(static_cast<hipStream_t>(hip_stream), DenseFwd{a->dtype, a->activation, a->m, a->k, a->n, a->x, a->ldx, a->kernel, a->ldk, a->bias, a->residual, a->ldr,
-                                                               a->y, a->ldy, a->save}, cus);
+  const DenseFwd f = dense_fwd_of(*a);
+  if (a->workspace) CHECK(check_workspace(who, a->workspace, a->workspace_bytes, (int64_t)dense_fwd_ws(f, cus)));
+  dense_forward(static_cast<hipStream_t>(hip_stream), f, cus);
   return launched(who);
 }
 

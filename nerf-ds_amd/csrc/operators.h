@@ -20,6 +20,7 @@ struct DenseFwd {
   const void* residual; long long ldr;      // [m][n] or nullptr (ldr 0: one row for all)
   void* y; long long ldy;                   // [m][n]
   void* save;                               // dense_save_bytes() for the backward pass, or nullptr
+  void* ws;                                 // dense_fwd_ws() bytes or nullptr
 };
 struct DenseBwd {
   int dtype, act;
@@ -36,6 +37,7 @@ struct DenseBwd {
 // What the forward leaves for the backward: relu one bit per element (row-major, rows of whole bytes), the smooth activations the pre-activation in
 // the tensors' type, no activation nothing.
 size_t dense_save_bytes(int dtype, int act, long long m, int n);
+size_t dense_fwd_ws(const DenseFwd& a, int num_cus);
 size_t dense_bwd_ws(const DenseBwd& a, int num_cus);
 void dense_forward(hipStream_t st, const DenseFwd& a, int num_cus);
 void dense_backward(hipStream_t st, const DenseBwd& a, int num_cus);

@@ -146,7 +146,8 @@ def dtype_code(dtype) -> int:
 class DenseForwardArgs(C.Structure):
   _fields_ = [('dtype', C.c_int32), ('activation', C.c_int32), ('m', C.c_int64), ('k', C.c_int32), ('n', C.c_int32),
               ('x', C.c_void_p), ('ldx', C.c_int64), ('kernel', C.c_void_p), ('ldk', C.c_int64), ('bias', C.c_void_p),
-              ('residual', C.c_void_p), ('ldr', C.c_int64), ('y', C.c_void_p), ('ldy', C.c_int64), ('save', C.c_void_p)]
+              ('residual', C.c_void_p), ('ldr', C.c_int64), ('y', C.c_void_p), ('ldy', C.c_int64), ('save', C.c_void_p),
+              ('workspace', C.c_void_p), ('workspace_bytes', C.c_int64)]
 
 
 class DenseBackwardArgs(C.Structure):
@@ -186,7 +187,7 @@ SYMBOLS = ('nerfds_abi_version', 'nerfds_struct_size', 'nerfds_precision_plan', 
            'nerfds_trainer_download', 'nerfds_trainer_upload', 'nerfds_trainer_reset_optimizer', 'nerfds_trainer_step', 'nerfds_trainer_apply', 'nerfds_trainer_clip_gradients', 'nerfds_trainer_target_norm',
            'nerfds_trainer_last_error', 'nerfds_trainer_debug_read', 'nerfds_trainer_nonfinite', 'nerfds_trainer_set_step', 'nerfds_trainer_get_step', 'nerfds_trainer_set_loss_scale_adjust', 'nerfds_trainer_set_numerics', 'nerfds_trainer_get_numerics', 'nerfds_trainer_overflow_sources', 'nerfds_trainer_forward', 'nerfds_render_rays_bwd',
            'nerfds_debug_lds_attr_first_use',
-           'nerfds_dense_save_bytes', 'nerfds_dense_backward_workspace', 'nerfds_dense_forward', 'nerfds_dense_backward', 'nerfds_layer_norm_forward',
+           'nerfds_dense_save_bytes', 'nerfds_dense_forward_workspace', 'nerfds_dense_backward_workspace', 'nerfds_dense_forward', 'nerfds_dense_backward', 'nerfds_layer_norm_forward',
            'nerfds_layer_norm_backward_workspace', 'nerfds_layer_norm_backward', 'nerfds_orthogonalize_workspace', 'nerfds_orthogonalize',
            'nerfds_trainer_set_optimizer', 'nerfds_trainer_leaf_optimizer')
 
@@ -237,6 +238,7 @@ def load():
   lib.nerfds_struct_size.argtypes = [C.c_int]
   lib.nerfds_struct_size.restype = C.c_int64
   lib.nerfds_dense_save_bytes.argtypes = [C.c_int32, C.c_int32, C.c_int64, C.c_int32]
+  lib.nerfds_dense_forward_workspace.argtypes = [C.c_int, C.POINTER(DenseForwardArgs)]
   lib.nerfds_dense_backward_workspace.argtypes = [C.c_int, C.POINTER(DenseBackwardArgs)]
   lib.nerfds_dense_forward.argtypes = [C.c_int, C.POINTER(DenseForwardArgs), C.c_void_p]
   lib.nerfds_dense_backward.argtypes = [C.c_int, C.POINTER(DenseBackwardArgs), C.c_void_p]
@@ -245,7 +247,7 @@ def load():
   lib.nerfds_layer_norm_backward.argtypes = [C.c_int, C.POINTER(LayerNormBackwardArgs), C.c_void_p]
   lib.nerfds_orthogonalize_workspace.argtypes = [C.POINTER(Matrix), C.c_int32]
   lib.nerfds_orthogonalize.argtypes = [C.c_int, C.c_int32, C.POINTER(Matrix), C.c_int32, C.c_int32, C.c_void_p, C.c_int64, C.c_void_p]
-  for f in (lib.nerfds_dense_save_bytes, lib.nerfds_dense_backward_workspace, lib.nerfds_layer_norm_backward_workspace, lib.nerfds_orthogonalize_workspace):
+  for f in (lib.nerfds_dense_save_bytes, lib.nerfds_dense_forward_workspace, lib.nerfds_dense_backward_workspace, lib.nerfds_layer_norm_backward_workspace, lib.nerfds_orthogonalize_workspace):
     f.restype = C.c_int64
   structs = {i: st for i, st in enumerate((ModelCfg, Weights, CameraStruct, Rays, Extra, Rand, Out))}
   structs.update({9: DenseForwardArgs, 10: DenseBackwardArgs, 11: LayerNormForwardArgs, 12: LayerNormBackwardArgs, 13: Matrix, 14: Optimizer})

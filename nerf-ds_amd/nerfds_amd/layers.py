@@ -96,8 +96,11 @@ def _dense_forward(x, kernel, bias, residual, activation, keep):
   save = None
   if keep and act:
     save = x.new_empty((m, (n + 7) // 8), dtype=torch.uint8) if activation == 'relu' else x.new_empty((m, n))
-  _call('nerfds_dense_forward', lib.nerfds_dense_forward, x, N.DenseForwardArgs(dt, act, m, k, n, x2.data_ptr(), ldx, w.data_ptr(), ldk, _ptr(bias), _ptr(r), ldr,
-                                                                              y.data_ptr(), n, _ptr(save)))
+  args = N.DenseForwardArgs(dt, act, m, k, n, x2.data_ptr(), ldx, w.data_ptr(), ldk, _ptr(bias), _ptr(r), ldr, y.data_ptr(), n, _ptr(save), None, 0)
+  if 8 < m < 32768:      # (outside: never a workspace)
+    _call_with_workspace('nerfds_dense_forward', lib.nerfds_dense_forward_workspace, lib.nerfds_dense_forward, x, args)
+  else:
+    _call('nerfds_dense_forward', lib.nerfds_dense_forward, x, args)
   return y, save
 
 

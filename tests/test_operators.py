@@ -171,6 +171,44 @@ def test_dense_wide_layers_over_many_rows(i, t):
   _gradients_together_and_apart(*WIDE[i], t)
 
 
+# few rows: the contraction of y (k) and of dx (n) split, each alone and both, ragged pieces
+FEW = [(9, 4096, 64, 'relu'), (12, 591, 2854, 'softplus'), (33, 2048, 300, 'none'), (64, 1000, 1000, 'gelu'), (130, 700, 40, 'silu'), (513, 3000, 20, 'relu'), (700, 24, 1999, 'sigmoid'), (10, 512, 513, 'relu')]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('t', [F32, F16, BF16], ids=['f32', 'f16', 'bf16'])
+@pytest.mark.parametrize('i', range(len(FEW)), ids=['%dx%dx%d-%s' % s for s in FEW])
+def test_dense_few_rows_over_long_contractions(i, t):
+  m, k, n, act = FEW[i]
+  grid = 0.25 if act == 'relu' else None
+  x, w, dy, b, r = dev(make(m, k, t=t, seed=6, grid=grid), make(k, n, t=t, seed=7, scale=1.0 if grid else k ** -0.5, grid=grid), make(m, n, t=t, seed=8),
+                       make(n, t=t, seed=9, grid=grid) if i % 3 else None, make(m, n, t=t, seed=10) if i % 2 else None)
+  want = dense64(x, w, b, r, act, dy)
+  y, saved = layers.dense_forward(x, w, b, act, r)
+  close(y, want['y'])
+  assert torch.equal(layers.dense_forward(x, w, b, act, r)[0], y)
+  for name, g in zip(('dx', 'dkernel', 'db'), layers.dense_backward(dy, x, w, saved, act)):
+    close(g, want[name], name)
+  close(layers.dense_backward(dy, x, w, saved, act, need_dkernel=False, need_dbias=False)[0], want['dx'])
+  # without a workspace, rows of y and the residual with a stride of their own; and what is no workspace
+  lib, code, wide = N.load(), N.dtype_code(t), torch.full((m, n + 3), -7.0, dtype=t, device='cuda')
+  a = N.DenseForwardArgs(code, N.ACTIVATIONS[act], m, k, n, x.data_ptr(), k, w.data_ptr(), n, b.data_ptr() if b is not None else None, r.data_ptr() if r is not None else None, n,
+                         wide.data_ptr(), n + 3, None)
+  st, index = torch.cuda.current_stream().cuda_stream, torch.cuda.current_device()
+  assert lib.nerfds_dense_forward(index, C.byref(a), st) == 0
+  close(wide[:, :n], want['y'])
+  nbytes = lib.nerfds_dense_forward_workspace(index, C.byref(a))
+  if nbytes > 0:
+    ws = torch.empty(nbytes + 256, dtype=torch.uint8, device='cuda')
+    wide.fill_(-7.0)
+    a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
+    assert lib.nerfds_dense_forward(index, C.byref(a), st) == 0
+    assert torch.equal(wide[:, :n], y) and bool((wide[:, n:] == -7.0).all())
+    for p, size in ((ws.data_ptr(), nbytes - 1), (ws.data_ptr() + 16, nbytes)):
+      a.workspace, a.workspace_bytes = p, size
+      assert lib.nerfds_dense_forward(index, C.byref(a), st) == -22
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize('t', [F16, BF16], ids=['f16', 'bf16'])
 @pytest.mark.parametrize('act', ['sigmoid', 'softplus', 'silu', 'gelu'])
