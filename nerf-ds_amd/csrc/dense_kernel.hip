@@ -34,6 +34,7 @@ struct GemmArgs {
   int tiles_n; long long tiles;
   long long lo;      // k_gemm: elements from dz to its second part, 0: it has one (data: operand a, weights: operand b)
   bool large;        // weights: k_tile takes it
+  void* dbias;       // weights: the column sums of b, by the one split there is (with more: colpart)
 };
 
 template <typename T> struct Shape;
@@ -242,7 +243,7 @@ __global__ __launch_bounds__(THREADS, 2) void k_gemm(const GemmArgs G) {
   f32x16 acc[2][2] = {};
   Gran<T> ra[TA::NG], rb[TB::NG];
   float cs[8] = {};
-  const bool sums = OUT == OUT_WEIGHTS && G.colpart != nullptr && m0 == 0;
+  const bool sums = OUT == OUT_WEIGHTS && (G.colpart != nullptr || G.dbias != nullptr) && m0 == 0;
   const T* pa = static_cast<const T*>(G.a);
   const T* pb = static_cast<const T*>(G.b);
   bool more = OUT != OUT_FORWARD && !MASK && sizeof(T) == 2 && G.lo != 0;
@@ -320,7 +321,8 @@ __global__ __launch_bounds__(THREADS, 2) void k_gemm(const GemmArgs G) {
       if (threadIdx.x < 128 && n0 + threadIdx.x < G.N) {
         float s = 0.f;
         for (int q = 0; q < 16; ++q) s += red[q * 128 + threadIdx.x];
-        G.colpart[blockIdx.y * ((G.N + 3) & ~3LL) + n0 + threadIdx.x] = s;
+        if (G.dbias != nullptr) static_cast<T*>(G.dbias)[n0 + threadIdx.x] = from_f32<T>(s);
+        else G.colpart[blockIdx.y * ((G.N + 3) & ~3LL) + n0 + threadIdx.x] = s;
       }
     }
   }
@@ -675,11 +677,11 @@ template <typename T> void backward_t(hipStream_t st, const DenseBwd& w, int num
     const long long kn = (long long)w.k * w.n;
     const size_t part_bytes = weight_part_bytes(w, s.count);
     G.part = w.dkernel && s.count > 1 ? reinterpret_cast<float*>(ws) : nullptr;
-    if (s.count == 1) { G.y = w.dkernel; G.ldy = w.n; }
     float* col = reinterpret_cast<float*>(ws + part_bytes);
-    G.colpart = w.dbias ? col : nullptr;
+    if (s.count == 1) { G.y = w.dkernel; G.ldy = w.n; G.dbias = w.dbias; }
+    else G.colpart = w.dbias ? col : nullptr;
     if (bits) launch<T, false, false, OUT_WEIGHTS, 2>(st, G, num_cus); else launch<T, false, false, OUT_WEIGHTS, 0>(st, G, num_cus);
-    sum_splits<T>(st, SplitSum{G.part, up(kn, 4) * 4, kn, G.part ? w.dkernel : nullptr}, SplitSum{col, up(w.n, 4) * 4, w.n, w.dbias}, s.count);
+    if (s.count > 1) sum_splits<T>(st, SplitSum{G.part, up(kn, 4) * 4, kn, w.dkernel}, SplitSum{col, up(w.n, 4) * 4, w.n, w.dbias}, s.count);
   }
 }
 
@@ -691,7 +693,7 @@ size_t dense_save_bytes(int dtype, int act, long long m, int n) {
 size_t dense_fwd_ws(const DenseFwd& a, int num_cus) { return row_part_bytes(row_splits(a.dtype, a.m, a.n, a.k, num_cus), a.m, a.n); }
 size_t dense_bwd_ws(const DenseBwd& a, int num_cus) {
   const Splits s = weight_splits(a, num_cus);
-  const size_t weights = a.dkernel != nullptr || a.dbias != nullptr ? weight_part_bytes(a, s.count) + aligned((size_t)s.count * up(a.n, 4) * 16) : 0;
+  const size_t weights = a.dkernel != nullptr || a.dbias != nullptr ? weight_part_bytes(a, s.count) + (s.count > 1 || both_at_once(a) ? aligned((size_t)s.count * up(a.n, 4) * 16) : 0) : 0;
   const size_t rows = a.dx != nullptr && !both_at_once(a) ? row_part_bytes(row_splits(a.dtype, a.m, a.k, a.n, num_cus), a.m, a.k) : 0;
   return dz_bytes(a) + (weights > rows ? weights : rows);
 }

@@ -175,7 +175,7 @@ template <typename T, typename GR, bool AC, bool BC, int OUT, int MASK, int ACT>
     long long tm, tn;
     tile_of(item - split * G.tiles, tiles_m, G.tiles_n, tm, tn);
     const long long m0 = tm * GR::BM, n0 = tn * GR::BN, c0 = split * G.cps, c1 = c0 + G.cps < G.C ? c0 + G.cps : G.C;
-    const bool sums = OUT == OUT_WEIGHTS && G.colpart != nullptr && tm == 0 && wm == 0;
+    const bool sums = OUT == OUT_WEIGHTS && (G.colpart != nullptr || G.dbias != nullptr) && tm == 0 && wm == 0;
     f32x16 acc[TM][TN] = {};
     f32x16 cs[OUT == OUT_WEIGHTS ? TN : 1] = {};
     for (long long c = c0; c < c1; c += BK) {
@@ -317,15 +317,17 @@ template <typename T, typename GR, bool AC, bool BC, int OUT, int MASK, int ACT>
     }
     if constexpr (OUT == OUT_WEIGHTS) {
       if (sums && (lane & 31) == 0) {
-        float* out = G.colpart + split * ((G.N + 3) & ~3LL);
 #pragma unroll
         for (int j = 0; j < TN; ++j)
 #pragma unroll
           for (int d = 0; d < 2; ++d) {
             const long long n = nw + 32 * j + 16 * d;
-            if (n < G.N)
+            float v[8];
 #pragma unroll
-              for (int e = 0; e < 8; ++e) out[n + e] = cs[j][8 * d + e];
+            for (int e = 0; e < 8; ++e) v[e] = cs[j][8 * d + e];
+            if (n >= G.N) continue;
+            if (G.dbias != nullptr) gran_store<T>(static_cast<T*>(G.dbias) + n, gran_pack<T>(v), 8);
+            else gran_store<float>(G.colpart + split * ((G.N + 3) & ~3LL) + n, gran_pack<float>(v), 8);
           }
       }
     }
