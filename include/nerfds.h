@@ -488,7 +488,7 @@ typedef struct nerfds_dense_forward_args {
 } nerfds_dense_forward_args;
 /* dz = dy act'(z); dx = dz kernel^T, dkernel = x^T dz, dbias = column sums of dz; the gradient of the residual is dy itself.  dx / dkernel / dbias may
  * be NULL (not computed).  For 16-bit tensors dz is rounded to their type between the slope and the products; none and
- * relu are exact, and up to 65536 elements dz goes into the products in two parts, without that rounding. */
+ * relu are exact, and up to 2^18 elements dz goes into the products in two parts, without that rounding. */
 typedef struct nerfds_dense_backward_args {
   int32_t dtype, activation;
   int64_t m;                          /* 0: dkernel and dbias are cleared */

@@ -39,9 +39,11 @@ struct BothArgs {
   void* dx; long long lddx;
   float* part; float* colpart;      // [grid][k n rounded up to 4], [grid][n rounded up to 4] (nullptr: no bias gradient)
   long long m; int k, n;
+  long long lo;      // elements from dz to its second part (LO)
 };
 
-template <typename T, int KP, int NP, bool MASK> __global__ __launch_bounds__(512) void k_both(const BothArgs G) {
+// LO: dz comes in two parts, and every stage twice, with one and the other
+template <typename T, int KP, int NP, bool MASK, bool LO> __global__ __launch_bounds__(512) void k_both(const BothArgs G) {
   typedef Both<KP, NP> S;
   constexpr int IPW = S::XI + S::YI + (MASK ? 1 : 0), RT = S::RT;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4, i16 = lane & 15;
@@ -63,6 +65,7 @@ template <typename T, int KP, int NP, bool MASK> __global__ __launch_bounds__(51
     }
 
   long long issued = blockIdx.x;
+  int part_issued = 0, part = 0;
   auto issue = [&](int slot) __attribute__((always_inline)) {
     const unsigned base = lds0 + slot * S::STAGE;
     const long long r0 = issued * S::ROWS;
@@ -76,14 +79,15 @@ template <typename T, int KP, int NP, bool MASK> __global__ __launch_bounds__(51
       }
     };
     tile(G.x, G.ldx, G.k, S::XI, KP / 8, base);
-    tile(G.dz, G.lddz, G.n, S::YI, NP / 8, base + S::XB);
+    tile(static_cast<const T*>(G.dz) + (LO && part_issued ? G.lo : 0), G.lddz, G.n, S::YI, NP / 8, base + S::XB);
     if constexpr (MASK) {      // NP / 32 dwords a row; the other waves fetch the same again, so that every wave counts alike
       constexpr int D = NP / 32, W = S::BITS / 256;
       const int d = 64 * (wave & (W - 1)) + lane, row = d / D, c = d % D;
       const bool in = r0 + row < G.m && 32 * c < G.n;
       dma4(in ? reinterpret_cast<const char*>(G.mask) + (r0 + row) * G.ldm + 4 * c : zeros, base + S::XB + S::YB + (wave & (W - 1)) * 256);
     }
-    issued += gridDim.x;
+    part_issued ^= 1;
+    if (!LO || !part_issued) issued += gridDim.x;
   };
 
   f32x16 acc[S::WK][S::WN] = {};
@@ -94,9 +98,11 @@ template <typename T, int KP, int NP, bool MASK> __global__ __launch_bounds__(51
 #pragma unroll
   for (int s = 0; s < S::RING - 1; ++s) issue(s);
   int slot = 0, done = 0;
-  for (long long stage = blockIdx.x; stage < stages; stage += gridDim.x) {
-    // this stage's DMA has landed: newer are two stages and, from the fourth stage on, the stores of three (the partial stage, which may store less, is the last)
-    if (done >= S::RING - 1 && stores) wait_loads<(S::RING - 2) * IPW + (S::RING - 1) * RT>(); else wait_loads<(S::RING - 2) * IPW>();
+  f32x4 d[RT][2];
+  for (long long stage = blockIdx.x; stage < stages;) {
+    // this stage's DMA has landed: newer are two stages and, from the fourth stage on, the stores of three (LO: of one at the least; the partial stage, which may
+    // store less, is the last)
+    if (done >= S::RING - 1 && stores) wait_loads<(S::RING - 2) * IPW + (LO ? 1 : S::RING - 1) * RT>(); else wait_loads<(S::RING - 2) * IPW>();
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
     issue((slot + S::RING - 1) % S::RING);
@@ -125,7 +131,10 @@ template <typename T, int KP, int NP, bool MASK> __global__ __launch_bounds__(51
         __builtin_amdgcn_sched_barrier(0);
       }
     }
-    f32x4 d[RT][2] = {};
+    if (!LO || part == 0) {
+#pragma unroll
+      for (int t = 0; t < RT; ++t) d[t][0] = d[t][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
 #pragma unroll
     for (int ks = 0; ks < S::KS; ++ks)
 #pragma unroll
@@ -148,6 +157,7 @@ template <typename T, int KP, int NP, bool MASK> __global__ __launch_bounds__(51
     }
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
+      if (LO && part == 0) break;
       const long long m = stage * S::ROWS + 16 * (row_tile + t) + i16;
       const int c = 32 * cols + 8 * q;
       const float v[8] = {d[t][0][0], d[t][0][1], d[t][0][2], d[t][0][3], d[t][1][0], d[t][1][1], d[t][1][2], d[t][1][3]};
@@ -155,6 +165,8 @@ template <typename T, int KP, int NP, bool MASK> __global__ __launch_bounds__(51
     }
     slot = slot + 1 == S::RING ? 0 : slot + 1;
     ++done;
+    part ^= 1;
+    if (!LO || part == 0) stage += gridDim.x;
   }
   wait_loads<0>();      // no DMA may be on its way into LDS that is used otherwise, or no longer this workgroup's
 

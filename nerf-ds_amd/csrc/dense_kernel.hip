@@ -476,24 +476,25 @@ bool stores_dz(const DenseBwd& w) {
   return true;
 }
 // Whether dz keeps its float32 value in two parts, which the products take one after the other: 16-bit layers so small that their time is latency, where the
-// rounding of dz would be the larger half of the gradients' error (45% more than the rounding of the results alone) and costs 1 - 4 us to avoid.
-bool two_parts(const DenseBwd& w) { return w.dtype != F32 && w.act != ACT_NONE && w.act != ACT_RELU && w.m <= 65536 / w.n; }
+// rounding of dz would be the larger half of the gradients' error (45% more than the rounding of the results alone, and for the few results of a
+// narrow layer by chance more) and costs 1.5 us (k_both, 64 x 64 at 4096 rows: 12.1 instead of 11.0) to 5 (256 x 256 at 1024 rows: 24 instead of 19) to avoid.
+bool two_parts(const DenseBwd& w) { return w.dtype != F32 && w.act != ACT_NONE && w.act != ACT_RELU && w.m <= (1 << 18) / w.n; }
 // Whether the operands of the weight gradient suit the tiles that come by DMA: whole, aligned granules, relu bits in whole dwords (a dz in the workspace is)
 bool weight_dma(const DenseBwd& w) {
-  if (w.dtype == F32 || w.k % 8 || w.n % 8 || !whole_granules(w.x, w.ldx) || two_parts(w)) return false;
+  if (w.dtype == F32 || w.k % 8 || w.n % 8 || !whole_granules(w.x, w.ldx)) return false;
   if (stores_dz(w)) return true;
   return whole_granules(w.dy, w.lddy) && (w.act != ACT_RELU || (w.n % 32 == 0 && reinterpret_cast<uintptr_t>(w.save) % 4 == 0));
 }
 // Whether the weight gradient takes the large tiles: from 2^34 multiply-adds on, or where the rows are so many that memory is the bound.  (k_gemm has more
 // workgroups in flight, k_tile the higher rate: 512 x 512 in bf16 at 32768 rows 41 us by k_gemm and 44 by k_tile, at 65536 rows 68 and 60; 1024 x 1024 at 8192
 // rows 38 and 42, at 32768 rows 106 and 91; 256 x 256 at 4096 rows 13 and 21)
-bool weight_tiles_large(const DenseBwd& w) { return weight_dma(w) && (w.m >= 131072 || w.m >= (1LL << 34) / ((long long)w.k * w.n)); }
+bool weight_tiles_large(const DenseBwd& w) { return weight_dma(w) && !two_parts(w) && (w.m >= 131072 || w.m >= (1LL << 34) / ((long long)w.k * w.n)); }
 
 // Whether both gradients come from one pass (k_both): a narrow layer in 16 bits, both wanted.  Up to 128 x 256 at any number of rows (128 x 128 in bf16: 9.7 us
 // instead of 6.1 + 8.5 at 512 rows, 20.5 instead of 11 + 21 at 65536), the larger ones where their parts of dkernel have rows enough behind them (256 x 256: 32
 // instead of 8.5 + 17 at 8192 rows, 40 instead of 15 + 24 at 32768, 47 instead of 23 + 33 at 65536, 213 instead of 119 + 130 at 524288).
 bool both_at_once(const DenseBwd& w) {
-  return w.dx != nullptr && w.dkernel != nullptr && w.k <= 256 && w.n <= 256 && (w.k * w.n <= 128 * 256 || w.m >= 32768) && weight_dma(w);
+  return w.dx != nullptr && w.dkernel != nullptr && w.k <= 256 && w.n <= 256 && ((w.k <= 128 || w.n <= 128) || (w.m >= 32768 && !two_parts(w))) && weight_dma(w);
 }
 
 constexpr int RESIDENT_M = 16384;
@@ -621,16 +622,17 @@ template <typename T> void forward_t(hipStream_t st, const DenseFwd& f, int num_
   launch<T, true, false, OUT_FORWARD, 0>(st, G, num_cus);
 }
 
-template <typename T, int KP, int NP, bool MASK> void launch_both(hipStream_t st, const BothArgs& G, int grid) {
-  auto kern = k_both<T, KP, NP, MASK>;
+template <typename T, int KP, int NP, bool MASK, bool LO> void launch_both(hipStream_t st, const BothArgs& G, int grid) {
+  auto kern = k_both<T, KP, NP, MASK, LO>;
   nerfds::allow_dynamic_lds(reinterpret_cast<const void*>(kern), Both<KP, NP>::LDS);
   hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(512), (Both<KP, NP>::LDS), st, G);
 }
-template <typename T, bool MASK> void launch_both_of(hipStream_t st, const BothArgs& G, int grid) {
-  if (G.k > 128 && G.n > 128) launch_both<T, 256, 256, MASK>(st, G, grid);
-  else if (G.k > 128) launch_both<T, 256, 128, MASK>(st, G, grid);
-  else if (G.n > 128) launch_both<T, 128, 256, MASK>(st, G, grid);
-  else launch_both<T, 128, 128, MASK>(st, G, grid);
+template <typename T, bool MASK, bool LO> void launch_both_of(hipStream_t st, const BothArgs& G, int grid) {
+  if (G.k > 128 && G.n > 128) {
+    if constexpr (!LO) launch_both<T, 256, 256, MASK, LO>(st, G, grid);      // (two parts: never of this size)
+  } else if (G.k > 128) launch_both<T, 256, 128, MASK, LO>(st, G, grid);
+  else if (G.n > 128) launch_both<T, 128, 256, MASK, LO>(st, G, grid);
+  else launch_both<T, 128, 128, MASK, LO>(st, G, grid);
 }
 
 template <typename T> void backward_t(hipStream_t st, const DenseBwd& w, int num_cus) {
@@ -653,8 +655,10 @@ template <typename T> void backward_t(hipStream_t st, const DenseBwd& w, int num
       const long long kn = (long long)w.k * w.n;
       float* part = reinterpret_cast<float*>(ws);
       float* col = reinterpret_cast<float*>(ws + weight_part_bytes(w, grid));
-      const BothArgs G{w.x, w.ldx, dz, lddz, w.kernel, w.ldk, bits, up(w.n, 8), w.dx, w.lddx, part, w.dbias ? col : nullptr, w.m, w.k, w.n};
-      if (bits) launch_both_of<T, true>(st, G, grid); else launch_both_of<T, false>(st, G, grid);
+      const BothArgs G{w.x, w.ldx, dz, lddz, w.kernel, w.ldk, bits, up(w.n, 8), w.dx, w.lddx, part, w.dbias ? col : nullptr, w.m, w.k, w.n, lo};
+      if (bits) launch_both_of<T, true, false>(st, G, grid);
+      else if (lo != 0) launch_both_of<T, false, true>(st, G, grid);
+      else launch_both_of<T, false, false>(st, G, grid);
       sum_splits<T>(st, SplitSum{part, up(kn, 4) * 4, kn, w.dkernel}, SplitSum{col, up(w.n, 4) * 4, w.n, w.dbias}, grid);
       return;
     }

@@ -213,7 +213,7 @@ def test_dense_few_rows_over_long_contractions(i, t):
 @pytest.mark.parametrize('t', [F16, BF16], ids=['f16', 'bf16'])
 @pytest.mark.parametrize('act', ['sigmoid', 'softplus', 'silu', 'gelu'])
 def test_dense_small_gradients_lose_only_their_own_rounding(act, t):
-  for m, k, n in ((2, 438, 13), (17, 2, 32), (1, 40, 8), (200, 300, 256), (16500, 16, 3), (5, 7, 9001)):
+  for m, k, n in ((2, 438, 13), (17, 2, 32), (1, 40, 8), (200, 300, 256), (16500, 16, 3), (5, 7, 9001), (3001, 64, 16), (130, 200, 128), (1000, 24, 200), (32768, 8, 8), (77, 128, 64)):
     # pre-activations that float32 sums exactly and the tensors' type holds, so that the saved ones are exact
     x, w, b, dy = dev(make(m, k, t=t, seed=1, grid=1.0), make(k, n, t=t, seed=2, scale=0.5, grid=0.25), make(n, t=t, seed=3, grid=0.25), make(m, n, t=t, seed=4))
     z = x.double() @ w.double() + b.double()
