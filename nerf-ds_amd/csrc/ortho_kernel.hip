@@ -129,6 +129,18 @@ OPS_DEV void split2(float v, _Float16& hi, _Float16& lo) {
   lo = (_Float16)(v - (float)hi);
 }
 
+OPS_DEV _Float16 half_of(const u32x2& v, int e) { return __builtin_bit_cast(_Float16, (uint16_t)(v[e >> 1] >> (16 * (e & 1)))); }
+OPS_DEV float f16_of(const u32x2& v, int e) { return (float)half_of(v, e); }
+OPS_DEV void split4(const float (&v)[4], u32x2 (&out)[2]) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    _Float16 hi, lo;
+    split2(v[e], hi, lo);
+    const unsigned h = __builtin_bit_cast(uint16_t, hi), l = __builtin_bit_cast(uint16_t, lo);
+    if (e & 1) { out[0][e >> 1] |= h << 16; out[1][e >> 1] |= l << 16; } else { out[0][e >> 1] = h; out[1][e >> 1] = l; }
+  }
+}
+
 // X0's planes, one 64 x 64 tile per workgroup
 template <typename T> __global__ __launch_bounds__(THREADS) void k_prepare(const Batch B) {
   __shared__ double red[THREADS];
@@ -150,30 +162,30 @@ template <typename T> __global__ __launch_bounds__(THREADS) void k_prepare(const
   _Float16* x = reinterpret_cast<_Float16*>(B.ws + M.ws + L.x(0));
   _Float16* xt = reinterpret_cast<_Float16*>(B.ws + M.ws + L.xt(0));
   const long long plane = (long long)L.np * L.mp;
-  for (int q = w; q < TILE; q += THREADS / 64) {
-    _Float16 hi, lo;
-    split2(tile[q][lane], hi, lo);
-    const long long e = (long long)(i0 + q) * L.mp + j0 + lane;
-    x[e] = hi;
-    x[plane + e] = lo;
-    split2(tile[lane][q], hi, lo);
-    const long long et = (long long)(j0 + q) * L.np + i0 + lane;
-    xt[et] = hi;
-    xt[plane + et] = lo;
+  // 8 elements of a row of X and of its transpose at a time (columns of 65 floats: 8 rows x 8 granules fall on all banks either way)
+  for (int e = threadIdx.x; e < TILE * 8; e += THREADS) {
+    const int q = e >> 3, g = 8 * (e & 7);
+    const long long at[2] = {(long long)(i0 + q) * L.mp + j0 + g, (long long)(j0 + q) * L.np + i0 + g};
+#pragma unroll
+    for (int turned = 0; turned < 2; ++turned) {
+      u32x4 plane_of[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = turned ? tile[g + 4 * h + k][q] : tile[q][g + 4 * h + k];
+        u32x2 pack[2];
+        split4(v, pack);
+#pragma unroll
+        for (int p = 0; p < 2; ++p) { plane_of[p][2 * h] = pack[p][0]; plane_of[p][2 * h + 1] = pack[p][1]; }
+      }
+      _Float16* out = (turned ? xt : x) + at[turned];
+      *reinterpret_cast<u32x4*>(out) = plane_of[0];
+      *reinterpret_cast<u32x4*>(out + plane) = plane_of[1];
+    }
   }
 }
 
-OPS_DEV _Float16 half_of(const u32x2& v, int e) { return __builtin_bit_cast(_Float16, (uint16_t)(v[e >> 1] >> (16 * (e & 1)))); }
-OPS_DEV float f16_of(const u32x2& v, int e) { return (float)half_of(v, e); }
-OPS_DEV void split4(const float (&v)[4], u32x2 (&out)[2]) {
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    _Float16 hi, lo;
-    split2(v[e], hi, lo);
-    const unsigned h = __builtin_bit_cast(uint16_t, hi), l = __builtin_bit_cast(uint16_t, lo);
-    if (e & 1) { out[0][e >> 1] |= h << 16; out[1][e >> 1] |= l << 16; } else { out[0][e >> 1] = h; out[1][e >> 1] = l; }
-  }
-}
 // from the accumulators (products of scaled planes) and the old value, at its own scale, to the new one (fused by hand: the compiler's choice could differ
 // between the kernels)
 OPS_DEV float gram_of(float acc) { return acc * (1.f / SX); }                                                        // A 2^15
