@@ -6,14 +6,17 @@
 // (up to 128 per lane), written once at the end, and so does the kernel (each wave the 32 rows of it that make its 32 columns of dx); at 256 x 256 only three
 // eighths of it find room there, the rest waits in LDS, 80 KB of it (half in registers spilled).  For 16 rows of 256 x 256 a wave does 16 MFMAs of 16 cycles for
 // dx and 8 of 32 for dkernel: 0.4 us per CU with two waves on a SIMD, a third of the time that the rows' 25 KB take memory.
-// Measured: 197 - 235 us by the card, and 12 to add the 256 parts of dkernel (memory's floor 174; apart 119 - 128 and 130 - 142).
+// Measured (relu): 197 - 235 us by the card, and 12 to add the 256 parts of dkernel (memory's floor 174; apart 119 - 128 and 130 - 142).
 #pragma once
 
-template <int KP_, int NP_> struct Both {
+// MODE: what dz is - BOTH_PLAIN: given; BOTH_RELU: dy by the relu bits; BOTH_SLOPE: dy act'(z), made in LDS from both
+enum { BOTH_PLAIN = 0, BOTH_RELU = 1, BOTH_SLOPE = 2 };
+template <int KP_, int NP_, int MODE> struct Both {
   static constexpr int KP = KP_, NP = NP_;      // k and n, padded to 128 or 256
   // rows per stage: 32, or 16 for the layer of 256 x 256, where KL of its contraction steps of 32 wait in LDS (KR are in registers)
   static constexpr bool FULL = KP == 256 && NP == 256;
-  static constexpr int ROWS = FULL ? 16 : 32, XB = ROWS * KP * 2, YB = ROWS * NP * 2, BITS = ROWS * NP / 8, STAGE = XB + YB + BITS, RING = 4;
+  static constexpr int ROWS = FULL ? 16 : 32, XB = ROWS * KP * 2, YB = ROWS * NP * 2, EXTRA = MODE == BOTH_RELU ? ROWS * NP / 8 : MODE == BOTH_SLOPE ? YB : 0,
+                       STAGE = XB + YB + EXTRA, RING = MODE == BOTH_SLOPE && NP == 256 ? 3 : 4;      // (z's rows beside dy's leave LDS for three stages)
   static constexpr int KS = NP / 32, KL = FULL ? 5 : 0, KR = KS - KL, LDS = RING * STAGE + 8 * 2 * KL * 1024;
   static constexpr int XI = XB / 8192, YI = YB / 8192;      // DMA instructions of a stage per wave
   // dkernel: GK x GN waves of (32 WK) x (32 WN); dx: RT tiles of 16 rows x 32 columns per wave
@@ -35,7 +38,7 @@ template <int KP_, int NP_> struct Both {
 
 struct BothArgs {
   const void* x; long long ldx; const void* dz; long long lddz; const void* kernel; long long ldk;
-  const unsigned char* mask; long long ldm;
+  const void* save; long long lds; int act;      // relu bits or z
   void* dx; long long lddx;
   float* part; float* colpart;      // [grid][k n rounded up to 4], [grid][n rounded up to 4] (nullptr: no bias gradient)
   long long m; int k, n;
@@ -43,9 +46,9 @@ struct BothArgs {
 };
 
 // LO: dz comes in two parts, and every stage twice, with one and the other
-template <typename T, int KP, int NP, bool MASK, bool LO> __global__ __launch_bounds__(512) void k_both(const BothArgs G) {
-  typedef Both<KP, NP> S;
-  constexpr int IPW = S::XI + S::YI + (MASK ? 1 : 0), RT = S::RT;
+template <typename T, int KP, int NP, int MODE, bool LO> __global__ __launch_bounds__(512) void k_both(const BothArgs G) {
+  typedef Both<KP, NP, MODE> S;
+  constexpr int IPW = S::XI + S::YI + (MODE == BOTH_RELU ? 1 : MODE == BOTH_SLOPE ? S::YI : 0), RT = S::RT;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4, i16 = lane & 15;
   const unsigned lds0 = __builtin_amdgcn_readfirstlane((unsigned)(size_t)(__attribute__((address_space(3))) char*)g_lds);
   const char* const zeros = reinterpret_cast<const char*>(g_zeros);
@@ -80,11 +83,12 @@ template <typename T, int KP, int NP, bool MASK, bool LO> __global__ __launch_bo
     };
     tile(G.x, G.ldx, G.k, S::XI, KP / 8, base);
     tile(static_cast<const T*>(G.dz) + (LO && part_issued ? G.lo : 0), G.lddz, G.n, S::YI, NP / 8, base + S::XB);
-    if constexpr (MASK) {      // NP / 32 dwords a row; the other waves fetch the same again, so that every wave counts alike
-      constexpr int D = NP / 32, W = S::BITS / 256;
+    if constexpr (MODE == BOTH_SLOPE) tile(G.save, G.lds, G.n, S::YI, NP / 8, base + S::XB + S::YB);
+    if constexpr (MODE == BOTH_RELU) {      // NP / 32 dwords a row; the other waves fetch the same again, so that every wave counts alike
+      constexpr int D = NP / 32, W = S::EXTRA / 256;
       const int d = 64 * (wave & (W - 1)) + lane, row = d / D, c = d % D;
       const bool in = r0 + row < G.m && 32 * c < G.n;
-      dma4(in ? reinterpret_cast<const char*>(G.mask) + (r0 + row) * G.ldm + 4 * c : zeros, base + S::XB + S::YB + (wave & (W - 1)) * 256);
+      dma4(in ? static_cast<const char*>(G.save) + (r0 + row) * G.lds + 4 * c : zeros, base + S::XB + S::YB + (wave & (W - 1)) * 256);
     }
     part_issued ^= 1;
     if (!LO || !part_issued) issued += gridDim.x;
@@ -109,23 +113,31 @@ template <typename T, int KP, int NP, bool MASK, bool LO> __global__ __launch_bo
     __builtin_amdgcn_sched_barrier(0);
     char* const x = g_lds + slot * S::STAGE;
     char* const y = x + S::XB;
-    if (MASK || G.colpart != nullptr) {
-      // relu bits multiply dz in place; the column sums are taken of what this thread brought in - the same 8 columns in every stage
+    if (MODE != BOTH_PLAIN || G.colpart != nullptr) {
+      // relu bits or slopes multiply dy in place; the column sums are taken of what this thread brought in - the same 8 columns in every stage
       const unsigned char* bits = reinterpret_cast<const unsigned char*>(y + S::YB);
 #pragma unroll
       for (int u = 0; u < S::YI; ++u) {
         const int s = (wave + 8 * u) * 64 + lane, row = s / (NP / 8), g = (s % (NP / 8)) ^ S::turn(row);
         Gran<T> v{*reinterpret_cast<const u32x4*>(y + s * 16)};
-        if constexpr (MASK) {
-          gran_mask<T>(v, bits[row * (NP / 8) + g]);
-          *reinterpret_cast<u32x4*>(y + s * 16) = v.v;
+        if constexpr (MODE == BOTH_RELU) gran_mask<T>(v, bits[row * (NP / 8) + g]);
+        if constexpr (MODE == BOTH_SLOPE) {      // (rounded to the tensors' type: the matrix pipe takes it in no other)
+          const Gran<T> z{*reinterpret_cast<const u32x4*>(y + S::YB + s * 16)};
+          float f[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) f[e] = gran_get<T>(z, e);
+          act_slopes<T>(f, G.act);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) f[e] *= gran_get<T>(v, e);
+          v = gran_pack<T>(f);
         }
+        if constexpr (MODE != BOTH_PLAIN) *reinterpret_cast<u32x4*>(y + s * 16) = v.v;
         if (G.colpart != nullptr) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) cs[e] += gran_get<T>(v, e);
         }
       }
-      if constexpr (MASK) {
+      if constexpr (MODE != BOTH_PLAIN) {
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);

@@ -497,6 +497,12 @@ bool both_at_once(const DenseBwd& w) {
   return w.dx != nullptr && w.dkernel != nullptr && w.k <= 256 && w.n <= 256 && ((w.k <= 128 || w.n <= 128) || (w.m >= 32768 && !two_parts(w))) && weight_dma(w);
 }
 
+// Whether k_both makes dz itself, from dy and z in LDS, instead of reading what k_dz wrote (524288 x 256 x 256 in bf16: 250 us instead of 331 with softplus, 297 instead
+// of 345 with gelu, whose erf is the bound then; 8192 x 128 x 128: 15 instead of 17)
+bool slopes_in_both(const DenseBwd& w) {
+  return w.act != ACT_NONE && w.act != ACT_RELU && both_at_once(w) && !two_parts(w) && whole_granules(w.dy, w.lddy) && whole_granules(w.save, w.n);
+}
+
 constexpr int RESIDENT_M = 16384;
 // The large tiles pay where they fill the card; with fewer the 128 x 128 tiles of k_gemm spread the work over more CUs
 bool large_tiles_fill(long long m, long long n, int num_cus) { return up(m, 256) * up(n, 128) >= num_cus / 2; }
@@ -535,7 +541,7 @@ Splits row_splits(int dtype, long long m, long long n, long long c, int num_cus)
 }
 size_t row_part_bytes(const Splits& s, long long m, long long n) { return s.count > 1 ? aligned((size_t)s.count * up(m * n, 4) * 16) : 0; }
 
-size_t dz_bytes(const DenseBwd& w) { return stores_dz(w) ? aligned((size_t)up(w.m * w.n, 8) * 8 * dtype_bytes(w.dtype) * (two_parts(w) ? 2 : 1)) : 0; }
+size_t dz_bytes(const DenseBwd& w) { return stores_dz(w) && !slopes_in_both(w) ? aligned((size_t)up(w.m * w.n, 8) * 8 * dtype_bytes(w.dtype) * (two_parts(w) ? 2 : 1)) : 0; }
 size_t weight_part_bytes(const DenseBwd& w, int splits) {      // (one split of the weight gradient alone writes the result itself)
   return splits > 1 || both_at_once(w) ? aligned((size_t)splits * up((long long)w.k * w.n, 4) * 16) : 0;
 }
@@ -622,24 +628,24 @@ template <typename T> void forward_t(hipStream_t st, const DenseFwd& f, int num_
   launch<T, true, false, OUT_FORWARD, 0>(st, G, num_cus);
 }
 
-template <typename T, int KP, int NP, bool MASK, bool LO> void launch_both(hipStream_t st, const BothArgs& G, int grid) {
-  auto kern = k_both<T, KP, NP, MASK, LO>;
-  nerfds::allow_dynamic_lds(reinterpret_cast<const void*>(kern), Both<KP, NP>::LDS);
-  hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(512), (Both<KP, NP>::LDS), st, G);
+template <typename T, int KP, int NP, int MODE, bool LO> void launch_both(hipStream_t st, const BothArgs& G, int grid) {
+  auto kern = k_both<T, KP, NP, MODE, LO>;
+  nerfds::allow_dynamic_lds(reinterpret_cast<const void*>(kern), Both<KP, NP, MODE>::LDS);
+  hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(512), (Both<KP, NP, MODE>::LDS), st, G);
 }
-template <typename T, bool MASK, bool LO> void launch_both_of(hipStream_t st, const BothArgs& G, int grid) {
+template <typename T, int MODE, bool LO> void launch_both_of(hipStream_t st, const BothArgs& G, int grid) {
   if (G.k > 128 && G.n > 128) {
-    if constexpr (!LO) launch_both<T, 256, 256, MASK, LO>(st, G, grid);      // (two parts: never of this size)
-  } else if (G.k > 128) launch_both<T, 256, 128, MASK, LO>(st, G, grid);
-  else if (G.n > 128) launch_both<T, 128, 256, MASK, LO>(st, G, grid);
-  else launch_both<T, 128, 128, MASK, LO>(st, G, grid);
+    if constexpr (!LO) launch_both<T, 256, 256, MODE, LO>(st, G, grid);      // (two parts: never of this size)
+  } else if (G.k > 128) launch_both<T, 256, 128, MODE, LO>(st, G, grid);
+  else if (G.n > 128) launch_both<T, 128, 256, MODE, LO>(st, G, grid);
+  else launch_both<T, 128, 128, MODE, LO>(st, G, grid);
 }
 
 template <typename T> void backward_t(hipStream_t st, const DenseBwd& w, int num_cus) {
   char* ws = static_cast<char*>(w.ws);
   const void* dz = w.dy;
   long long lddz = w.lddy;
-  const bool stored = stores_dz(w);
+  const bool stored = stores_dz(w) && !slopes_in_both(w);
   const long long lo = two_parts(w) ? up(w.m * w.n, 8) * 8 : 0;
   if (stored) {
     const long long grans = w.m * up(w.n, 8), want = up(grans, 256);
@@ -655,10 +661,11 @@ template <typename T> void backward_t(hipStream_t st, const DenseBwd& w, int num
       const long long kn = (long long)w.k * w.n;
       float* part = reinterpret_cast<float*>(ws);
       float* col = reinterpret_cast<float*>(ws + weight_part_bytes(w, grid));
-      const BothArgs G{w.x, w.ldx, dz, lddz, w.kernel, w.ldk, bits, up(w.n, 8), w.dx, w.lddx, part, w.dbias ? col : nullptr, w.m, w.k, w.n, lo};
-      if (bits) launch_both_of<T, true, false>(st, G, grid);
-      else if (lo != 0) launch_both_of<T, false, true>(st, G, grid);
-      else launch_both_of<T, false, false>(st, G, grid);
+      const BothArgs G{w.x, w.ldx, dz, lddz, w.kernel, w.ldk, w.save, w.act == ACT_RELU ? up(w.n, 8) : w.n, w.act, w.dx, w.lddx, part, w.dbias ? col : nullptr, w.m, w.k, w.n, lo};
+      if (bits) launch_both_of<T, BOTH_RELU, false>(st, G, grid);
+      else if (slopes_in_both(w)) launch_both_of<T, BOTH_SLOPE, false>(st, G, grid);
+      else if (lo != 0) launch_both_of<T, BOTH_PLAIN, true>(st, G, grid);
+      else launch_both_of<T, BOTH_PLAIN, false>(st, G, grid);
       sum_splits<T>(st, SplitSum{part, up(kn, 4) * 4, kn, w.dkernel}, SplitSum{col, up(w.n, 4) * 4, w.n, w.dbias}, grid);
       return;
     }

@@ -150,7 +150,8 @@ def test_dense_at_sizes_with_many_tiles_and_splits(i, t):
 # both gradients in one pass: each width class, a last stage of a few rows or of one, several rounds of the ring of stages, one workgroup
 BOTH = [(32768, 256, 256, 'relu'), (150001, 256, 256, 'relu'), (140003, 160, 136, 'gelu'), (140033, 256, 96, 'relu'), (90001, 200, 64, 'none'), (90007, 64, 256, 'relu'), (33000, 128, 200, 'silu'),
         (100001, 96, 128, 'relu'), (70000, 128, 8, 'none'),
-        (1, 256, 256, 'relu'), (63, 256, 256, 'none'), (65, 128, 160, 'relu'), (500, 8, 32, 'relu')]
+        (1, 256, 256, 'relu'), (63, 256, 256, 'none'), (65, 128, 160, 'relu'), (500, 8, 32, 'relu'),
+        (100003, 256, 64, 'softplus'), (50001, 64, 64, 'sigmoid'), (40000, 256, 256, 'silu'), (70001, 104, 256, 'gelu')]
 
 
 @pytest.mark.gpu
